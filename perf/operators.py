@@ -161,10 +161,11 @@ def _offsets(lengths):
 
 
 def _quantise(x):
-    """Rows of x as e4m3 codes and the scale of each: code * scale is the value."""
+    """Rows of x as e4m3 codes and the scale of each: code * scale is the value.  x * E4M3_MAX is exact
+    (x has 11 bits at most) and the quotient's one rounding keeps a tie between two codes a tie."""
     x = x.float()
     most = x.abs().amax(-1, keepdim=True).clamp_min(TINY)
-    return (x * (E4M3_MAX / most)).to(torch.float8_e4m3fn), (most / E4M3_MAX).squeeze(-1)
+    return (x * E4M3_MAX / most).to(torch.float8_e4m3fn), (most / E4M3_MAX).squeeze(-1)
 
 
 def prepare(case, seed):
@@ -620,8 +621,9 @@ def _exact_cache(st):
             held[page, :, at] = rows
             out[x + "_cache"] = held
             continue
-        scale = torch.clamp(rows.abs().max(-1, keepdim=True).values, min=TINY) / E4M3_MAX
-        y = rows / scale
+        most = torch.clamp(rows.abs().max(-1, keepdim=True).values, min=TINY)
+        scale = most / E4M3_MAX
+        y = rows * E4M3_MAX / most
         step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)
         out[x] = torch.round(y / step) * step * scale
         held = torch.zeros(st[x + "_scale"].shape, device=DEV, dtype=torch.float64)
