@@ -6,7 +6,8 @@
  * returns 0, or a nonzero code with a message from vdk_last_error().  Nothing
  * here allocates device memory except vdk_malloc, vdk_fbank (the workspace that
  * vdk_fbank_ex takes from its caller), vdk_res2_block in place on clips of
- * several time tiles (vdk_res2_block_out does not) and the opt-in tile tuning.
+ * several time tiles (vdk_res2_block_out does not), vdk_attn_plan_create (a
+ * layout's tables) and the opt-in tile tuning.
  * Shapes are checked on the host before any launch.
  *
  * Layouts: PCM [B][n] f32; FBank features feat-major [B][n_mels][T] f32 (the
@@ -582,6 +583,133 @@ int vdk_time_mean_acc(const void* d_x, int x_f32, int batch, int T, int C, float
  * vdk_time_mean_acc call per state in turn. */
 int vdk_time_mean_states(const void* d_x, size_t state_stride, int n_states, int batch, int T, int C,
                          const float* weights, float* d_out, void* stream);
+
+/* ---- attention with a learned position bias over packed clips ----
+ * For query i and key j of a clip, r = j - (i + past) and past = keys - queries:
+ *   x = scale * q_i . k_j,  s = cap * tanh(x / cap) + bias[head][clamp(r, -R, R) + R]
+ *   (cap = 0: s = x + bias; no bias pointer: no bias),
+ *   o_i = sum_j softmax_j(s) v_j,  lse_i = log sum_j exp(s).
+ * With `causal` query i sees the keys with r <= 0 and the clip's first `prefix`
+ * keys, else all keys of its clip.  A row that sees nothing (no key, or a bias
+ * of -inf at each) gives o = 0 and lse = -inf.  A NaN or an infinity in a key
+ * or value reaches every query of the same 32 that sees a key of its 64-key
+ * tile; clips never reach each other.
+ *
+ * The clips lie one after the other: clip c has queries q_offsets[c] ..
+ * q_offsets[c + 1] - 1 and keys kv_offsets[c] .. kv_offsets[c + 1] - 1 (host
+ * arrays of n_clips + 1, from 0, never falling; a clip may be empty).  Heads:
+ * n_heads a multiple of n_kv_heads, head h reads key head h / (n_heads /
+ * n_kv_heads); head_dim 64 or 128.  A plan holds one such layout and its work
+ * lists on the current device; prefix [n_clips] may be NULL (0) and needs
+ * causal.  A plan is read only: calls on several streams may share it. */
+enum { VDK_F16 = 0, VDK_BF16 = 1 };
+typedef struct vdk_attn_plan vdk_attn_plan;
+int  vdk_attn_plan_create(int n_clips, const long long* q_offsets, const long long* kv_offsets, int n_heads,
+                          int n_kv_heads, int head_dim, int causal, const long long* prefix, vdk_attn_plan** plan);
+void vdk_attn_plan_destroy(vdk_attn_plan* plan);
+
+/* Pointers are 16-byte aligned; strides count elements between tokens (*_tok,
+ * head_dim .. 2^22) and heads (*_head), multiples of 8, so q, k and v may be
+ * slices of one projection's output.  dist_bias [n_heads][2 bias_radius + 1]
+ * f32 (may be NULL; bias_radius 1 .. 4096) must hold no NaN.  o has the inputs'
+ * type, o_f32 [total_q][n_heads][head_dim] f32 (the same values unrounded; the
+ * backward pass reads them) and lse [n_heads][total_q] f32 may be NULL. */
+typedef struct {
+    int dtype;                    /* VDK_F16 or VDK_BF16: q, k, v, o and the gradients */
+    float scale, cap;             /* scale > 0; cap >= 0, 0: none */
+    const void* q; long long q_tok, q_head;
+    const void* k; long long k_tok, k_head;
+    const void* v; long long v_tok, v_head;
+    const float* dist_bias; int bias_radius;
+    void* o; long long o_tok, o_head;
+    float* o_f32;
+    float* lse;
+} vdk_relpos_attn;
+int vdk_relpos_attention(const vdk_attn_plan* plan, const vdk_relpos_attn* a, void* stream);
+
+/* Gradients of vdk_relpos_attention from the output's gradient d_o; a as in the
+ * forward call, its o_f32 and lse filled by it.  dq, dk, dv (the inputs' type,
+ * shared heads summed) and d_dist_bias [n_heads][2 bias_radius + 1] f32 (may be
+ * NULL) are overwritten.  Every sum has a fixed order: equal calls give equal
+ * bits.  Rows whose scores all lie below -1e30 count as rows that see nothing. */
+typedef struct {
+    const void* d_o; long long do_tok, do_head;
+    void* dq; long long dq_tok, dq_head;
+    void* dk; long long dk_tok, dk_head;
+    void* dv; long long dv_tok, dv_head;
+    float* d_dist_bias;
+    void* work; size_t work_bytes;
+} vdk_relpos_attn_grad;
+size_t vdk_relpos_attention_backward_workspace_size(const vdk_attn_plan* plan, int bias_radius);
+int vdk_relpos_attention_backward(const vdk_attn_plan* plan, const vdk_relpos_attn* a, const vdk_relpos_attn_grad* g,
+                                  void* stream);
+
+/* The bias of each distance from a table of buckets, dist_bias[h][r + R] =
+ * table[bucket(r)][h] for r = -R .. R, and its gradient, d_table[b][h] = the sum
+ * of d_dist_bias[h][r + R] over the distances of bucket b (f64 sums).  Of the
+ * n_buckets half (bidirectional; n_buckets even) serve keys after the query,
+ * bucket n_buckets / 2 upwards; without, all keys after the query share bucket
+ * 0.  Within a half of n: the first n / 2 hold one distance each, the others
+ * ranges that widen with its logarithm up to max_distance, from which all share
+ * the last: n / 2 + floor(log(d / (n / 2)) / log(max_distance / (n / 2)) * (n - n / 2)).
+ * n_buckets 4 .. 1024 (2 .. 512 a half), max_distance > n / 2, R 1 .. 4096. */
+int vdk_rel_bias_expand(const float* d_table, int n_buckets, int n_heads, int bidirectional, int max_distance,
+                        int bias_radius, float* d_dist_bias, void* stream);
+int vdk_rel_bias_reduce(const float* d_dist_grad, int n_buckets, int n_heads, int bidirectional, int max_distance,
+                        int bias_radius, float* d_table_grad, void* stream);
+
+/* ---- paged key-value cache of streams, and one new frame's attention over it ----
+ * k and v [n_pages][n_kv_heads][page_size][head_dim], dense and 16-byte aligned:
+ * VDK_KV_16 in the type `dtype`, VDK_KV_E4M3 as e4m3 codes with one f32 scale a
+ * row, k_scale and v_scale [n_pages][n_kv_heads][page_size] (value = code *
+ * scale).  page_size 16, 32, 64 or 128, head_dim 64 or 128.  Device-side
+ * findings are or-ed into *d_status (one int the caller clears; may be NULL). */
+enum { VDK_KV_16 = 0, VDK_KV_E4M3 = 1 };
+enum { VDK_STATUS_BAD_SLOT = 1, VDK_STATUS_BAD_PAGE = 2, VDK_STATUS_BAD_LENGTH = 4 };
+typedef struct {
+    int dtype, format, n_pages, page_size, n_kv_heads, head_dim;
+    void *k, *v;
+    float *k_scale, *v_scale;
+} vdk_kv_cache;
+/* Rows of n tokens written to their slots (slot = page * page_size + place in
+ * the page, 64-bit, device): k and v [n][n_kv_heads][head_dim] of the type
+ * dtype, strides in elements, multiples of 8.  Quantised rows: m = max(|x|,
+ * 2^-64), scale = m / 448, code = the e4m3 value nearest to 448 x / m, ties to
+ * even; a row that holds a NaN or an infinity reads back as NaN.  A negative slot is skipped; a slot
+ * past the cache is skipped and sets VDK_STATUS_BAD_SLOT; of two tokens with
+ * one slot either may stay. */
+int vdk_kv_cache_write(const vdk_kv_cache* c, const long long* d_slots, long long n, const void* d_k, long long k_tok,
+                       long long k_head, const void* d_v, long long v_tok, long long v_head, int* d_status,
+                       void* stream);
+/* The rows of n slots as values of the type dtype, [n][n_kv_heads][head_dim];
+ * the rows of negative and of bad slots are zeros (a bad one sets the status). */
+int vdk_kv_cache_read(const vdk_kv_cache* c, const long long* d_slots, long long n, void* d_k, long long k_tok,
+                      long long k_head, void* d_v, long long v_tok, long long v_head, int* d_status, void* stream);
+
+/* One query a stream over its cached keys: key j of stream s lies in page
+ * block_table[s][j / page_size] (int32 [n_seqs][max_pages]), j < seq_lens[s]
+ * (int32); the query is the last of them, r = j - (seq_lens[s] - 1), with the
+ * scores of vdk_relpos_attention.  q and o [n_seqs][n_q_heads][head_dim] of the
+ * type dtype (strides in elements, multiples of 8), lse [n_seqs][n_q_heads] f32
+ * (may be NULL).  max_len: an upper bound of seq_lens, at most max_pages *
+ * page_size; it sets how the work is split.  A length outside 0 .. max_len is
+ * clamped and sets VDK_STATUS_BAD_LENGTH; keys of a page outside the cache are
+ * hidden and set VDK_STATUS_BAD_PAGE.  A stream without keys gives o = 0 and
+ * lse = -inf.  What pages hold past a stream's length is not looked at.  work:
+ * vdk_paged_attention_workspace_size bytes, 16-byte aligned (may be 0). */
+typedef struct {
+    int n_seqs, n_q_heads, max_pages, max_len;
+    const void* q; long long q_seq, q_head;
+    const int *block_table, *seq_lens;
+    float scale, cap;
+    const float* dist_bias; int bias_radius;
+    void* o; long long o_seq, o_head;
+    float* lse;
+    void* work; size_t work_bytes;
+    int* status;
+} vdk_paged_attn;
+size_t vdk_paged_attention_workspace_size(const vdk_kv_cache* c, const vdk_paged_attn* a);
+int vdk_paged_attention(const vdk_kv_cache* c, const vdk_paged_attn* a, void* stream);
 
 #ifdef __cplusplus
 }

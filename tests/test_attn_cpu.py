@@ -1,0 +1,169 @@
+"""Refusals of the attention and cache entry points: all are found on the host,
+before any device work, so they need no GPU."""
+import ctypes as C
+
+import pytest
+
+from vdamd import lib
+
+L = lib.lib()
+P = 4096   # an aligned address that no call here reaches
+
+
+def err():
+    return L.vdk_last_error().decode()
+
+
+def plan(q=(0, 5, 9), kv=(0, 5, 9), H=4, kvh=2, D=64, **kw):
+    return lib.AttnPlan(list(q), list(kv), H, kvh, D, **kw)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(q=(1, 5, 9)), "start at 0"), (dict(q=(0, 9, 5)), "must not fall"), (dict(kv=(0, -1, 9)), "must not fall"),
+    (dict(D=80), "head_dim"), (dict(H=3), "n_heads"), (dict(kvh=0), "n_heads"), (dict(H=0), "n_heads"),
+    (dict(prefix=[1, 0]), "causal"), (dict(causal=True, prefix=[6, 0]), "prefix"), (dict(causal=True, prefix=[-1, 0]), "prefix"),
+    (dict(q=(0, 5, 1 << 31), kv=(0, 5, 1 << 31)), "2^30"),
+])
+def test_plan_refusals(kw, word):
+    with pytest.raises(lib.VdkError, match=word.replace("^", "\\^")):
+        plan(**kw)
+
+
+def test_plan_of_nothing_and_bad_lists():
+    lib.AttnPlan([0], [0], 1, 1, 64).close()
+    with pytest.raises(ValueError):
+        lib.AttnPlan([0, 1], [0], 1, 1, 64)
+    assert L.vdk_attn_plan_create(1, None, None, 1, 1, 64, 0, None, None) != 0
+    L.vdk_attn_plan_destroy(None)
+
+
+def attn(**kw):
+    a = lib.RelposAttn()
+    a.dtype, a.scale, a.cap = lib.F16, 0.125, 0.0
+    for x in ("q", "k", "v", "o"):
+        setattr(a, x, P)
+        setattr(a, x + "_tok", 64 * 4)
+        setattr(a, x + "_head", 64)
+    a.lse, a.o_f32 = P, P
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD_ATTN = [
+    (dict(dtype=2), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(cap=-1.0), "cap"), (dict(cap=float("inf")), "cap"), (dict(cap=1e-4), "cap"),
+    (dict(dist_bias=P, bias_radius=0), "bias_radius"), (dict(dist_bias=P, bias_radius=4097), "bias_radius"),
+    (dict(dist_bias=P + 2, bias_radius=4), "misaligned"), (dict(lse=P + 1), "misaligned"), (dict(o_f32=P + 4), "misaligned"),
+    (dict(q=None), "q is NULL"), (dict(k=P + 8), "k must be 16"), (dict(v_tok=68), "strides of v"),
+    (dict(o_tok=32), "strides of o"), (dict(q_head=12), "strides of q"), (dict(k_tok=1 << 23), "strides of k"),
+]
+
+
+@pytest.mark.parametrize("kw,word", BAD_ATTN)
+def test_attention_refusals(kw, word):
+    p = plan()
+    assert L.vdk_relpos_attention(p.ptr, attn(**kw), None) != 0
+    assert word in err()
+    g = lib.RelposAttnGrad()
+    assert L.vdk_relpos_attention_backward(p.ptr, attn(**kw), g, None) != 0
+
+
+def test_attention_refuses_missing_arguments():
+    p = plan()
+    assert L.vdk_relpos_attention(None, attn(), None) != 0 and "NULL" in err()
+    assert L.vdk_relpos_attention(p.ptr, None, None) != 0 and "NULL" in err()
+    assert L.vdk_relpos_attention_backward(p.ptr, attn(), None, None) != 0
+    empty = lib.AttnPlan([0, 0], [0, 0], 4, 2, 64)
+    assert L.vdk_relpos_attention(empty.ptr, attn(q=None, k=None, v=None, o=None), None) == 0
+
+
+def test_backward_workspace():
+    p = plan()
+    n = L.vdk_relpos_attention_backward_workspace_size(p.ptr, 0)
+    assert n >= 4 * 9 * 4
+    assert L.vdk_relpos_attention_backward_workspace_size(p.ptr, 16) >= n + 4 * 2 * 33 * 4
+    assert L.vdk_relpos_attention_backward_workspace_size(None, 0) == 0 and "NULL" in err()
+    assert L.vdk_relpos_attention_backward_workspace_size(p.ptr, -1) == 0 and "bias_radius" in err()
+
+
+@pytest.mark.skipif(L.vdk_device_count() > 0, reason="a plan made here has its tables")
+def test_a_plan_without_a_gpu_is_refused():
+    p = plan()
+    assert L.vdk_relpos_attention(p.ptr, attn(), None) != 0 and "without a GPU" in err()
+
+
+@pytest.mark.parametrize("args,word", [
+    ((None, 32, 4, 1, 128, 128, P), "NULL"), ((P, 3, 4, 0, 128, 128, P), "n_buckets"), ((P, 33, 4, 1, 128, 128, P), "n_buckets"),
+    ((P, 1026, 4, 1, 4000, 128, P), "n_buckets"), ((P, 513, 4, 0, 4000, 128, P), "n_buckets"), ((P, 32, 0, 1, 128, 128, P), "n_heads"),
+    ((P, 32, 4, 1, 8, 128, P), "max_distance"), ((P, 32, 4, 1, 128, 0, P), "bias_radius"), ((P, 32, 4, 1, 128, 5000, P), "bias_radius"),
+])
+def test_bucket_refusals(args, word):
+    for f in (L.vdk_rel_bias_expand, L.vdk_rel_bias_reduce):
+        assert f(*args, None) != 0
+        assert word in err()
+
+
+def cache(**kw):
+    c = lib.KvCache()
+    c.dtype, c.format, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = lib.BF16, lib.KV_E4M3, 4, 16, 2, 64
+    c.k = c.v = c.k_scale = c.v_scale = P
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+BAD_CACHE = [(dict(dtype=5), "dtype"), (dict(format=2), "format"), (dict(page_size=24), "page_size"), (dict(head_dim=96), "head_dim"),
+             (dict(n_pages=0), "empty"), (dict(n_kv_heads=0), "empty"), (dict(k=None), "NULL"), (dict(v_scale=None), "NULL"),
+             (dict(v=P + 8), "aligned")]
+
+
+@pytest.mark.parametrize("kw,word", BAD_CACHE)
+def test_cache_refusals(kw, word):
+    c = cache(**kw)
+    for f in (L.vdk_kv_cache_write, L.vdk_kv_cache_read):
+        assert f(c, P, 3, P, 128, 64, P, 128, 64, None, None) != 0
+        assert word in err()
+    assert L.vdk_paged_attention(c, paged(), None) != 0
+    assert word in err()
+
+
+def test_cache_row_refusals():
+    for f in (L.vdk_kv_cache_write, L.vdk_kv_cache_read):
+        assert f(None, P, 3, P, 128, 64, P, 128, 64, None, None) != 0 and "NULL" in err()
+        assert f(cache(), P, -1, P, 128, 64, P, 128, 64, None, None) != 0 and "negative" in err()
+        assert f(cache(), None, 3, P, 128, 64, P, 128, 64, None, None) != 0 and "slots" in err()
+        assert f(cache(), P, 3, None, 128, 64, P, 128, 64, None, None) != 0 and "k is NULL" in err()
+        assert f(cache(), P, 3, P, 128, 64, P + 2, 128, 64, None, None) != 0 and "v:" in err()
+        assert f(cache(), P, 3, P, 130, 64, P, 128, 64, None, None) != 0 and "k:" in err()
+        assert f(cache(), P, 0, None, 0, 0, None, 0, 0, None, None) == 0
+
+
+def paged(**kw):
+    a = lib.PagedAttn()
+    a.n_seqs, a.n_q_heads, a.max_pages, a.max_len = 3, 4, 10, 160
+    a.q = a.o = a.block_table = a.seq_lens = a.lse = P
+    a.q_seq = a.o_seq = 256
+    a.q_head = a.o_head = 64
+    a.scale = 0.125
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(n_seqs=-1), "negative"), (dict(max_len=-1), "negative"), (dict(n_q_heads=3), "n_q_heads"), (dict(n_q_heads=0), "n_q_heads"),
+    (dict(max_len=161), "block table"), (dict(scale=0.0), "scale"), (dict(cap=-2.0), "cap"), (dict(dist_bias=P, bias_radius=0), "bias_radius"),
+    (dict(q=None), "q is NULL"), (dict(o=P + 4), "o:"), (dict(seq_lens=None), "NULL"), (dict(block_table=None), "NULL"),
+    (dict(seq_lens=P + 2), "misaligned"), (dict(q_seq=260), "q:"),
+    (dict(max_pages=4000, max_len=64000), "workspace"),
+])
+def test_paged_refusals(kw, word):
+    assert L.vdk_paged_attention(cache(), paged(**kw), None) != 0
+    assert word in err()
+
+
+def test_paged_of_no_streams():
+    assert L.vdk_paged_attention(cache(), paged(n_seqs=0, q=None, o=None, block_table=None, seq_lens=None), None) == 0
+    assert L.vdk_paged_attention_workspace_size(cache(), paged()) == 0
+    assert L.vdk_paged_attention_workspace_size(cache(), paged(max_pages=4000, max_len=64000)) > 0

@@ -1,0 +1,258 @@
+"""The paged cache (vdk_kv_cache_write, vdk_kv_cache_read) and vdk_paged_attention
+against their formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import attn_ref as ref
+from gpu_util import announce, device_ok
+from vdamd import lib
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not device_ok(), reason="no HIP device")]
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+class Cache:
+    def __init__(self, pages, page, kv, D, dtype, quant, fill=None):
+        self.t, self.quant, self.page, self.kv, self.D, self.pages = TYPES[dtype], quant, page, kv, D, pages
+        shape = (pages, kv, page, D)
+        self.k, self.v = ((torch.full(shape, 0x7f if fill else 0, dtype=torch.uint8, device="cuda") if quant else
+                           torch.full(shape, float("nan") if fill else 0.0, dtype=self.t, device="cuda")) for _ in range(2))
+        self.ks, self.vs = ((torch.full(shape[:3], float("nan") if fill else 0.0, device="cuda") if quant else None)
+                            for _ in range(2))
+        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        d = self.d = lib.KvCache()
+        d.dtype, d.format = (lib.F16 if dtype == "f16" else lib.BF16), (lib.KV_E4M3 if quant else lib.KV_16)
+        d.n_pages, d.page_size, d.n_kv_heads, d.head_dim = pages, page, kv, D
+        d.k, d.v = self.k.data_ptr(), self.v.data_ptr()
+        if quant:
+            d.k_scale, d.v_scale = self.ks.data_ptr(), self.vs.data_ptr()
+
+    def write(self, slots, k, v):
+        s = slots.cuda()
+        lib.check(lib.lib().vdk_kv_cache_write(self.d, s.data_ptr(), len(slots), k.data_ptr(), k.stride(0), k.stride(1),
+                                               v.data_ptr(), v.stride(0), v.stride(1), self.status.data_ptr(), None))
+        torch.cuda.synchronize()
+
+    def read(self, slots):
+        s = slots.cuda()
+        k, v = (torch.full((len(slots), self.kv + 1, self.D), 7.0, dtype=self.t, device="cuda") for _ in range(2))
+        lib.check(lib.lib().vdk_kv_cache_read(self.d, s.data_ptr(), len(slots), k.data_ptr(), k.stride(0), k.stride(1),
+                                              v.data_ptr(), v.stride(0), v.stride(1), self.status.data_ptr(), None))
+        torch.cuda.synchronize()
+        assert (k[:, self.kv] == 7).all() and (v[:, self.kv] == 7).all()
+        return k[:, :self.kv], v[:, :self.kv]
+
+    def flags(self):
+        x = int(self.status.item())
+        self.status.zero_()
+        return x
+
+
+def e4m3(y):
+    """The nearest e4m3 value, ties to even (64 bits)."""
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)
+    return torch.round(y / step) * step
+
+
+@pytest.mark.parametrize("quant", [True, False], ids=["e4m3", "16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,page,kv,D", [(1, 16, 1, 64), (37, 32, 12, 64), (200, 64, 3, 128), (129, 128, 2, 64)])
+def test_rows_written_and_read_back(n, page, kv, D, dtype, quant):
+    announce(f"kv cache n={n} page={page} kv={kv} D={D} {dtype} quant={quant}")
+    pages = -(-n // page) + 3
+    c = Cache(pages, page, kv, D, dtype, quant)
+    g = torch.Generator().manual_seed(n)
+    kv2 = torch.randn(n, 2 * kv, D, generator=g)
+    kv2[0, 0] = torch.arange(D) - D / 2            # small whole numbers: quotients that are ties
+    kv2[0, -1] = 0.0
+    if n > 2:
+        kv2[1] *= 2.0 ** -12
+        kv2[2] *= 2.0 ** 7
+        kv2[3, 0] = 0.0
+        kv2[3, 0, 5] = 2.0 ** -14
+    both = kv2.to(TYPES[dtype]).cuda()
+    k, v = both[:, :kv], both[:, kv:]
+    slots = torch.randperm(pages * page, generator=g)[:n]
+    c.write(slots, k, v)
+    back = c.read(slots)
+    assert c.flags() == 0
+    for x, y, held, scales in ((k, back[0], c.k, c.ks), (v, back[1], c.v, c.vs)):
+        rows = x.double().cpu()
+        if not quant:
+            assert torch.equal(y, x)
+            assert torch.equal(held[slots // page, :, slots % page], x)
+            continue
+        m = rows.abs().amax(-1, keepdim=True).clamp_min(2.0 ** -64)
+        code = e4m3(rows * 448 / m)
+        got = held[slots // page, :, slots % page].view(torch.float8_e4m3fn).float().double().cpu()
+        assert torch.equal(got, code)
+        scale = scales[slots // page, :, slots % page].cpu()
+        assert torch.equal(scale, (m.float() / 448).squeeze(-1))
+        assert torch.equal(y.cpu(), (code.float() * scale[..., None]).to(x.dtype))
+    other = torch.ones(pages * page, dtype=torch.bool)
+    other[slots] = False
+    untouched = torch.arange(pages * page)[other]
+    assert (c.k[untouched // page, :, untouched % page].float() == 0).all()
+
+
+@pytest.mark.parametrize("quant", [True, False], ids=["e4m3", "16"])
+def test_skipped_and_bad_slots_and_rows_that_are_not_finite(quant):
+    c = Cache(2, 16, 2, 64, "f16", quant)
+    x = torch.randn(6, 2, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    x[2, 0, 3], x[3, 1, 63] = float("inf"), float("nan")
+    slots = torch.tensor([5, -1, 6, 7, 32, 1 << 40])
+    c.write(slots, x, x)
+    assert c.flags() == lib.STATUS_BAD_SLOT
+    k, v = c.read(slots)
+    assert c.flags() == lib.STATUS_BAD_SLOT
+    assert (k[[1, 4, 5]] == 0).all() and (v[[1, 4, 5]] == 0).all()
+    if quant:
+        assert torch.isnan(k[2, 0]).all() and torch.isnan(v[3, 1]).all()
+        assert torch.isfinite(k[2, 1]).all() and torch.isfinite(v[3, 0]).all()
+    else:
+        assert torch.equal(k[3].view(torch.int16), x[3].view(torch.int16))
+    c.write(slots[:0], x[:0], x[:0])
+
+
+def paged(c, q, table, lens, max_len, cap=0.0, dist=None, status=True):
+    L = lib.lib()
+    n, H, D = q.shape
+    a = lib.PagedAttn()
+    a.n_seqs, a.n_q_heads, a.max_pages, a.max_len = n, H, table.shape[1], max_len
+    a.q, a.q_seq, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    t, ln = table.int().cuda(), lens.int().cuda()
+    a.block_table, a.seq_lens = t.data_ptr(), ln.data_ptr()
+    a.scale, a.cap = 1 / math.sqrt(D), cap
+    if dist is not None:
+        d = dist.cuda()
+        a.dist_bias, a.bias_radius = d.data_ptr(), (dist.shape[1] - 1) // 2
+    o = torch.full((n, H, D), float("nan"), dtype=q.dtype, device="cuda")
+    lse = torch.full((n, H), float("nan"), device="cuda")
+    a.o, a.o_seq, a.o_head, a.lse = o.data_ptr(), H * D, D, lse.data_ptr()
+    size = L.vdk_paged_attention_workspace_size(c.d, a)
+    work = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device="cuda")
+    a.work, a.work_bytes, a.status = work.data_ptr(), size, c.status.data_ptr() if status else None
+    lib.check(L.vdk_paged_attention(c.d, a, None))
+    torch.cuda.synchronize()
+    first = o.clone()
+    o.zero_()
+    lib.check(L.vdk_paged_attention(c.d, a, None))
+    torch.cuda.synchronize()
+    assert torch.equal(o.view(torch.int16), first.view(torch.int16))
+    return o, lse
+
+
+def streams(lens, page, kv, D, dtype, quant, H, seed=0):
+    """A cache full of NaN but for the streams' own rows, pages in random order; the rows as they read back."""
+    g = torch.Generator().manual_seed(seed)
+    per = [-(-n // page) for n in lens]
+    c = Cache(sum(per) + 2, page, kv, D, dtype, quant, fill=True)
+    order = torch.randperm(c.pages, generator=g)
+    table = torch.full((len(lens), max(per + [1])), -7)   # entries past a stream's pages are never read
+    at, rows = 0, []
+    for i, (n, p) in enumerate(zip(lens, per)):
+        table[i, :p] = order[at:at + p]
+        at += p
+        if n == 0:
+            rows.append((torch.zeros(0, kv, D),) * 2)
+            continue
+        j = torch.arange(n)
+        slots = table[i, j // page] * page + j % page
+        k, v = (torch.randn(n, kv, D, generator=g).to(c.t).cuda() for _ in range(2))
+        c.write(slots, k, v)
+        if quant:
+            rows.append(tuple((held[slots // page, :, slots % page].view(torch.float8_e4m3fn).float().double()
+                               * s[slots // page, :, slots % page].double()[..., None]).cpu()
+                              for held, s in ((c.k, c.ks), (c.v, c.vs))))
+        else:
+            rows.append((k.double().cpu(), v.double().cpu()))
+    q = (torch.randn(len(lens), H + 1, D, generator=g) * 1.2).to(c.t).cuda()[:, :H]
+    return c, table, rows, q
+
+
+def expected(rows, q, lens, cap, dist, dtype):
+    """o, lse and their bounds: those of attn_ref with the value's scale (one more rounding of P)."""
+    o, lse, to, tl = [], [], [], []
+    for i, (k, v) in enumerate(rows):
+        out, tol = ref.attend(q[i:i + 1].cpu().double(), k.double(), v.double(), [0, 1], [0, lens[i]], 1 / math.sqrt(q.shape[2]), cap,
+                              dist, False, None)
+        u, fl = ref.half_step(dtype), ref.floor16(dtype)
+        H, G = q.shape[1], q.shape[1] // k.shape[1]
+        P = torch.zeros(q.shape[1], q.shape[2], dtype=torch.float64)
+        for h in range(H):
+            kk, vv = k[:, h // G].double(), v[:, h // G].double()
+            s, _, _, _ = ref.scores(q[i, h:h + 1].cpu().double(), kk, 1 / math.sqrt(q.shape[2]), cap,
+                                    None if dist is None else dist[h].double(),
+                                    0 if dist is None else (dist.shape[1] - 1) // 2, lens[i] - 1, torch.tensor([lens[i]]))
+            p, _ = ref.softmax(s)
+            P[h] = (p @ vv.abs())[0] + lens[i] * fl * (vv.abs().amax(0) if lens[i] else 0)
+        o.append(out["o"][0])
+        lse.append(out["lse"][:, 0])
+        # attend() above saw 64-bit tensors: its own bound has the scores' part, u and the floor come from here
+        to.append(tol["o"][0] + 2 * u * P + u * out["o"][0].abs() + fl)
+        tl.append(tol["lse"][:, 0])
+    return [torch.stack(x) for x in (o, lse, to, tl)]
+
+
+PAGED = [
+    dict(lens=[1], page=16, kv=1, D=64, dtype="f16", quant=False, H=1),
+    dict(lens=[0, 1, 15, 16, 17, 33], page=16, kv=2, D=64, dtype="bf16", quant=True, H=2, R=4),
+    dict(lens=[500], page=16, kv=12, D=64, dtype="f16", quant=False, H=12, R=128),
+    dict(lens=[100, 129, 513], page=32, kv=2, D=128, dtype="f16", quant=True, H=16, cap=30.0),
+    dict(lens=[1300, 5, 0, 700], page=64, kv=2, D=128, dtype="bf16", quant=True, H=8, cap=30.0, R=20),
+    dict(lens=[2500], page=128, kv=1, D=64, dtype="f16", quant=True, H=32),
+    dict(lens=[2500, 31], page=64, kv=1, D=128, dtype="bf16", quant=False, H=20, cap=200.0, R=800),
+    dict(lens=[640, 641], page=128, kv=4, D=128, dtype="f16", quant=False, H=4),
+]
+
+
+@pytest.mark.parametrize("case", PAGED, ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()).replace(" ", ""))
+def test_one_frame_over_the_cache(case):
+    announce(f"paged {case}")
+    case = dict(case)
+    R, cap = case.pop("R", 0), case.pop("cap", 0.0)
+    c, table, rows, q = streams(**case)
+    dist = torch.randn(case["H"], 2 * R + 1, generator=torch.Generator().manual_seed(3)) if R else None
+    o, lse = paged(c, q, table, torch.tensor(case["lens"]), max(case["lens"]), cap, dist)
+    assert c.flags() == 0
+    wo, wl, to, tl = expected(rows, q, case["lens"], cap, dist, c.t)
+    ref.check(o, wo, to, "o")
+    ref.check(lse, wl, tl, "lse")
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -14, 2.0 ** 9])
+def test_values_far_from_one_keep_their_precision(scale):
+    """f16 rows of very small or large values: a value's scale times p would leave f16."""
+    c, table, _, q = streams([300], 32, 2, 64, "f16", True, 4)
+    g = torch.Generator().manual_seed(9)
+    k = torch.randn(300, 2, 64, generator=g).half().cuda()
+    v = (torch.randn(300, 2, 64, generator=g) * scale).half().cuda()
+    j = torch.arange(300)
+    slots = table[0, j // 32] * 32 + j % 32
+    c.write(slots, k, v)
+    rows = [tuple((held[slots // 32, :, slots % 32].view(torch.float8_e4m3fn).float().double()
+                   * s[slots // 32, :, slots % 32].double()[..., None]).cpu() for held, s in ((c.k, c.ks), (c.v, c.vs)))]
+    o, lse = paged(c, q, table, torch.tensor([300]), 300)
+    wo, wl, to, tl = expected(rows, q, [300], 0.0, None, c.t)
+    ref.check(o, wo, to, "o")
+    ref.check(lse, wl, tl, "lse")
+
+
+def test_bad_pages_and_lengths_are_reported_and_hidden():
+    c, table, rows, q = streams([100, 64, 40], 16, 2, 64, "f16", True, 4)
+    good = table.clone()
+    table[0, 2] = c.pages          # keys 32 .. 47 of the first stream
+    table[1, 0] = -1               # keys 0 .. 15 of the second
+    o, lse = paged(c, q, table, torch.tensor([100, 64, 4000]), 112)
+    assert c.flags() == lib.STATUS_BAD_PAGE | lib.STATUS_BAD_LENGTH
+    keep = [torch.tensor([j for j in range(100) if not 32 <= j < 48]), torch.arange(16, 64)]
+    part = [tuple(x[j] for x in r) for r, j in zip(rows, keep)]
+    wo, wl, to, tl = expected(part, q[:2], [84, 48], 0.0, None, c.t)
+    ref.check(o[:2], wo, to, "o")
+    ref.check(lse[:2], wl, tl, "lse")
+    o, lse = paged(c, q, good, torch.tensor([100, -3, 40]), 112)
+    assert c.flags() == lib.STATUS_BAD_LENGTH
+    assert (o[1] == 0).all() and torch.isneginf(lse[1]).all()
+    paged(c, q, table, torch.tensor([100, 64, 40]), 112, status=False)

@@ -1,0 +1,294 @@
+"""vdk_relpos_attention, its backward pass and the bias by buckets against their
+formulas in 64 bits (attn_ref.py), elementwise within bounds counted there."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import attn_ref as ref
+from gpu_util import announce, device_ok
+from vdamd import lib
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not device_ok(), reason="no HIP device")]
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def offsets(n):
+    at = [0]
+    for x in n:
+        at.append(at[-1] + x)
+    return at
+
+
+class Layer:
+    """One packed layout on the GPU: inputs as slices of a wider tensor, outputs, descriptors."""
+
+    def __init__(self, nq, H, kv, D, dtype, nk=None, R=0, cap=0.0, causal=False, prefix=None, seed=0, scale=None,
+                 train=True):
+        self.q_at, self.kv_at = offsets(nq), offsets(nk or nq)
+        self.H, self.kv, self.D, self.R, self.cap, self.causal, self.prefix = H, kv, D, R, cap, causal, prefix
+        self.scale = scale or 1 / math.sqrt(D)
+        t = self.t = TYPES[dtype]
+        g = torch.Generator().manual_seed(seed)
+        n, m = self.q_at[-1], self.kv_at[-1]
+        self.q = (torch.randn(n, H + 1, D, generator=g) * 1.2).to(t)[:, :H]
+        kvs = torch.randn(m, 2 * kv, D, generator=g).to(t)
+        self.k, self.v = kvs[:, :kv], kvs[:, kv:]
+        self.do = (torch.randn(n, H, D, generator=g) * 0.05).to(t)
+        self.dist = torch.randn(H, 2 * R + 1, generator=g) if R else None
+
+    def up(self):
+        """To the GPU with the strides kept."""
+        def put(x):
+            if x is None:
+                return None
+            base = torch.zeros(x.shape[0], x.stride(0) // x.shape[2] if x.shape[0] else 1, x.shape[2], dtype=x.dtype,
+                               device="cuda")
+            y = base[:, :x.shape[1]]
+            y.copy_(x)
+            return y
+        self.g = {n: put(getattr(self, n)) for n in ("q", "k", "v", "do")}
+        self.g["dist"] = None if self.dist is None else self.dist.cuda()
+        a = self.a = lib.RelposAttn()
+        a.dtype, a.scale, a.cap = (lib.F16 if self.t == torch.float16 else lib.BF16), self.scale, self.cap
+        for x in ("q", "k", "v"):
+            y = self.g[x]
+            setattr(a, x, y.data_ptr())
+            setattr(a, x + "_tok", y.stride(0))
+            setattr(a, x + "_head", y.stride(1))
+        if self.R:
+            a.dist_bias, a.bias_radius = self.g["dist"].data_ptr(), self.R
+        n, m, H, D = self.q_at[-1], self.kv_at[-1], self.H, self.D
+        nan = float("nan")
+        self.o = torch.full((n, H, D), nan, dtype=self.t, device="cuda")
+        self.o32 = torch.full((n, H, D), nan, device="cuda")
+        self.lse = torch.full((H, n), nan, device="cuda")
+        a.o, a.o_tok, a.o_head = self.o.data_ptr(), H * D, D
+        a.lse = self.lse.data_ptr()
+        self.plan = lib.AttnPlan(self.q_at, self.kv_at, H, self.kv, D, causal=self.causal, prefix=self.prefix)
+        return self
+
+    def forward(self, train=False):
+        self.a.o_f32 = self.o32.data_ptr() if train else None
+        lib.check(lib.lib().vdk_relpos_attention(self.plan.ptr, self.a, None))
+        torch.cuda.synchronize()
+        return {"o": self.o, "lse": self.lse}
+
+    def backward(self):
+        L, H, D = lib.lib(), self.H, self.D
+        n, m = self.q_at[-1], self.kv_at[-1]
+        nan = float("nan")
+        self.dq = torch.full((n, H, D), nan, dtype=self.t, device="cuda")
+        self.dk, self.dv = (torch.full((m, self.kv, D), nan, dtype=self.t, device="cuda") for _ in range(2))
+        b = lib.RelposAttnGrad()
+        b.d_o, b.do_tok, b.do_head = self.g["do"].data_ptr(), self.g["do"].stride(0), self.g["do"].stride(1)
+        b.dq, b.dq_tok, b.dq_head = self.dq.data_ptr(), H * D, D
+        b.dk, b.dk_tok, b.dk_head = self.dk.data_ptr(), self.kv * D, D
+        b.dv, b.dv_tok, b.dv_head = self.dv.data_ptr(), self.kv * D, D
+        out = {"dq": self.dq, "dk": self.dk, "dv": self.dv}
+        if self.R:
+            self.ddist = torch.full((H, 2 * self.R + 1), nan, device="cuda")
+            b.d_dist_bias = self.ddist.data_ptr()
+            out["ddist"] = self.ddist
+        size = L.vdk_relpos_attention_backward_workspace_size(self.plan.ptr, self.R)
+        self.work = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device="cuda")
+        b.work, b.work_bytes = self.work.data_ptr(), size
+        lib.check(L.vdk_relpos_attention_backward(self.plan.ptr, self.a, b, None))
+        torch.cuda.synchronize()
+        return out
+
+    def reference(self, grad=False):
+        return ref.attend(self.q, self.k, self.v, self.q_at, self.kv_at, self.scale, self.cap, self.dist, self.causal,
+                          self.prefix, self.do if grad else None)
+
+
+FORWARD = [
+    # clips, heads, key heads, D, type, and what differs
+    dict(nq=[1], H=1, kv=1, D=64, dtype="f16"),
+    dict(nq=[0, 1, 2, 31, 0, 32, 33], H=2, kv=2, D=64, dtype="bf16", R=3),
+    dict(nq=[63, 64, 65, 127], H=4, kv=2, D=64, dtype="f16", R=40),
+    dict(nq=[149], H=12, kv=12, D=64, dtype="f16", R=128),
+    dict(nq=[128, 129, 200], H=4, kv=1, D=128, dtype="bf16", R=800),
+    dict(nq=[300, 17], H=8, kv=1, D=64, dtype="bf16", cap=20.0),
+    dict(nq=[130, 5], H=2, kv=2, D=128, dtype="f16", cap=300.0, R=9),
+    dict(nq=[70, 257], H=4, kv=2, D=64, dtype="f16", causal=True),
+    dict(nq=[70, 257, 3], H=4, kv=4, D=128, dtype="f16", causal=True, prefix=[0, 100, 3], R=20, cap=50.0),
+    dict(nq=[1, 40, 100], nk=[301, 45, 163], H=4, kv=2, D=128, dtype="bf16", causal=True, cap=30.0),
+    dict(nq=[1, 33, 2], nk=[500, 700, 64], H=2, kv=1, D=64, dtype="f16", causal=True, R=64, prefix=[5, 0, 64]),
+    dict(nq=[40, 7, 9], nk=[10, 0, 64], H=2, kv=2, D=64, dtype="f16", causal=True),      # rows that see nothing
+    dict(nq=[40, 7], nk=[10, 0], H=2, kv=1, D=128, dtype="bf16", R=2),
+]
+
+
+def ident(c):
+    return "-".join(f"{k}={v}" for k, v in c.items()).replace(" ", "")
+
+
+@pytest.mark.parametrize("train", [False, True], ids=["serve", "train"])
+@pytest.mark.parametrize("case", FORWARD, ids=ident)
+def test_forward(case, train):
+    announce(f"relpos forward {case} train={train}")
+    x = Layer(**case)
+    want, tol = x.reference()
+    got = x.up().forward(train)
+    for n in ("o", "lse"):
+        ref.check(got[n], want[n], tol[n], n)
+    if train:
+        u = ref.half_step(x.t)
+        ref.check(x.o32, want["o"], tol["o"] - u * want["o"].abs(), "o_f32")
+
+
+GRAD = [
+    dict(nq=[1], H=1, kv=1, D=64, dtype="f16", R=1),
+    dict(nq=[0, 2, 31, 32, 33], H=2, kv=2, D=64, dtype="bf16", R=3),
+    dict(nq=[63, 64, 65], H=4, kv=2, D=64, dtype="f16", R=40),
+    dict(nq=[149, 60], H=4, kv=4, D=64, dtype="f16", R=128),
+    dict(nq=[129, 200], H=4, kv=1, D=128, dtype="bf16", R=800),
+    dict(nq=[300, 17], H=8, kv=1, D=64, dtype="bf16", cap=20.0),
+    dict(nq=[130, 5], H=2, kv=2, D=128, dtype="f16", cap=300.0, R=9),
+    dict(nq=[70, 257], H=4, kv=2, D=64, dtype="f16", causal=True),
+    dict(nq=[70, 257, 3], H=4, kv=4, D=128, dtype="f16", causal=True, prefix=[0, 100, 3], R=20, cap=50.0),
+    dict(nq=[1, 40, 100], nk=[301, 45, 163], H=4, kv=2, D=128, dtype="bf16", causal=True, cap=30.0, R=33),
+    dict(nq=[40, 7, 9], nk=[10, 0, 64], H=2, kv=2, D=64, dtype="f16", causal=True, R=5),
+    dict(nq=[0, 40], nk=[70, 0], H=2, kv=1, D=64, dtype="bf16", R=5),
+]
+
+
+@pytest.mark.parametrize("case", GRAD, ids=ident)
+def test_backward(case):
+    announce(f"relpos backward {case}")
+    x = Layer(**case)
+    want, tol = x.reference(grad=True)
+    x.up().forward(True)
+    got = x.backward()
+    for n, y in got.items():
+        ref.check(y, want[n], tol[n], n)
+    again = {n: y.clone() for n, y in got.items()}
+    for n, y in x.backward().items():
+        assert torch.equal(y, again[n]), f"{n}: another call, other bits"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_gradients_of_very_small_and_uneven_output_gradients(dtype):
+    """Rows of dO that differ by 2^20: the 16-bit dS keep each row's precision (dq) and each block's (dk)."""
+    x = Layer([70, 40], 2, 1, 64, dtype, R=16)
+    f = torch.ones(110)
+    f[3::7] = 2.0 ** -10
+    f[40:] = 2.0 ** -12
+    x.do = (x.do.float() * f[:, None, None]).to(x.t)
+    want, tol = x.reference(grad=True)
+    x.up().forward(True)
+    for n, y in x.backward().items():
+        ref.check(y, want[n], tol[n], n)
+
+
+def test_gradients_against_differences():
+    """d loss / d q, k, v, bias along random directions against central differences of the formulas' loss."""
+    x = Layer([50, 33], 4, 2, 64, "f16", R=12, cap=25.0, causal=True, prefix=[4, 0])
+    x.up().forward(True)
+    got = {n: y.double().cpu() for n, y in x.backward().items()}
+    g = torch.Generator().manual_seed(5)
+
+    def loss(q, k, v, dist):
+        o, _ = ref.attend(q.double(), k.double(), v.double(), x.q_at, x.kv_at, x.scale, x.cap, dist, True, x.prefix)
+        return float((o["o"] * x.do.double()).sum())
+    base = {"q": x.q.double(), "k": x.k.double(), "v": x.v.double(), "dist": x.dist.double()}
+    for n in base:
+        d = torch.randn(base[n].shape, generator=g, dtype=torch.float64)
+        h = 1e-4
+        hi, lo = (loss(**dict(base, **{n: base[n] + s * h * d})) for s in (1, -1))
+        want, have = (hi - lo) / (2 * h), float((got["d" + n] * d).sum())
+        # each of the N outputs is off by 2^-11 (its rounding) and about as much (16-bit P, dS), at random signs
+        bound = 8 * 2.0 ** -11 * float((got["d" + n] * d).square().sum().sqrt()) + 1e-6 * abs(want)
+        assert abs(want - have) <= bound, (n, want, have, bound)
+
+
+def test_biases_of_minus_infinity_and_of_the_lowest_value():
+    """-inf hides keys, whole rows too; the type's lowest value hides keys but leaves a row of it alone an even mean."""
+    x = Layer([100], 2, 2, 64, "f16", R=30)
+    x.dist[0, :20] = -math.inf                     # keys 11 and more back
+    x.dist[1, :] = -math.inf                       # every key: rows that see nothing
+    y = Layer([100], 2, 2, 64, "f16", R=30)
+    low = torch.finfo(torch.float32).min
+    y.dist[0, :20] = low
+    y.dist[1, :] = low
+    for z in (x, y):
+        want, tol = z.reference(grad=z is x)
+        got = z.up().forward(True)
+        ref.check(got["o"], want["o"], tol["o"], "o")
+        ref.check(got["lse"], want["lse"], tol["lse"], "lse")
+    assert (x.o[:, 1] == 0).all() and torch.isneginf(x.lse[1]).all()
+    want, tol = x.reference(grad=True)
+    for n, v in x.backward().items():
+        ref.check(v, want[n], tol[n], n)
+
+
+def test_clips_do_not_reach_each_other():
+    x = Layer([100, 33, 70], 2, 2, 64, "bf16", R=8)
+    want, tol = x.reference(grad=True)
+    for y in (x.q, x.k, x.v):
+        y[100:133] = float("nan")                  # the middle clip
+    x.up().forward(True)
+    got = dict(x.backward(), o=x.o)
+    keep = [i for i in range(203) if not 100 <= i < 133]
+    for n in ("o", "dq", "dk", "dv"):
+        ref.check(got[n][keep], want[n][keep], tol[n][keep], n)
+
+
+def test_same_results_on_another_stream_and_in_a_graph():
+    x = Layer([149, 60], 4, 2, 64, "f16", R=128, cap=30.0).up()
+    x.forward(True)
+    first = dict(x.forward(True), **x.backward())
+    first = {n: y.clone() for n, y in first.items()}
+    s = torch.cuda.Stream()
+    L = lib.lib()
+    b = lib.RelposAttnGrad()
+    n, m, H, D = x.q_at[-1], x.kv_at[-1], x.H, x.D
+    b.d_o, b.do_tok, b.do_head = x.g["do"].data_ptr(), H * D, D
+    b.dq, b.dq_tok, b.dq_head = x.dq.data_ptr(), H * D, D
+    b.dk, b.dk_tok, b.dk_head = x.dk.data_ptr(), x.kv * D, D
+    b.dv, b.dv_tok, b.dv_head = x.dv.data_ptr(), x.kv * D, D
+    b.d_dist_bias, b.work, b.work_bytes = x.ddist.data_ptr(), x.work.data_ptr(), x.work.numel()
+    outs = {"o": x.o, "lse": x.lse, "dq": x.dq, "dk": x.dk, "dv": x.dv, "ddist": x.ddist}
+
+    def call():
+        p = torch.cuda.current_stream().cuda_stream
+        lib.check(L.vdk_relpos_attention(x.plan.ptr, x.a, p))
+        lib.check(L.vdk_relpos_attention_backward(x.plan.ptr, x.a, b, p))
+    with torch.cuda.stream(s):
+        for y in outs.values():
+            y.zero_()
+        call()
+    torch.cuda.synchronize()
+    for n_, y in outs.items():
+        assert torch.equal(y, first[n_]), n_
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        for y in outs.values():
+            y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for n_, y in outs.items():
+            assert torch.equal(y, first[n_]), n_
+        x.forward(True)
+
+
+BUCKETS = [(32, 1, 128, 128), (320, 1, 800, 800), (32, 0, 128, 200), (5, 0, 7, 30), (4, 1, 3, 1), (1024, 1, 4000, 4096)]
+
+
+@pytest.mark.parametrize("nb,both,far,R", BUCKETS)
+def test_bias_by_buckets_and_its_gradient(nb, both, far, R):
+    H, L = 5, lib.lib()
+    g = torch.Generator().manual_seed(nb)
+    table, grad = torch.randn(nb, H, generator=g).cuda(), torch.randn(H, 2 * R + 1, generator=g).cuda()
+    dist, dtable = torch.empty(H, 2 * R + 1, device="cuda"), torch.full((nb, H), float("nan"), device="cuda")
+    lib.check(L.vdk_rel_bias_expand(table.data_ptr(), nb, H, both, far, R, dist.data_ptr(), None))
+    lib.check(L.vdk_rel_bias_reduce(grad.data_ptr(), nb, H, both, far, R, dtable.data_ptr(), None))
+    torch.cuda.synchronize()
+    at = torch.tensor([ref.bucket(r, nb, both, far) for r in range(-R, R + 1)])
+    assert torch.equal(dist.cpu(), table.cpu()[at].t())
+    want = torch.zeros(nb, H, dtype=torch.float64).index_add_(0, at, grad.cpu().double().t())
+    ref.check(dtable, want, ref.F32 * want.abs() + 1e-12, "table gradient")   # 64-bit sums, one rounding

@@ -1,0 +1,216 @@
+// attn.hpp - what the attention kernels share: 16-bit types and their MFMAs,
+// swizzled LDS tiles, the score map, and a packed layout's plan.
+#pragma once
+
+#include <cfloat>
+#include <cmath>
+#include <vector>
+
+#include "common.hpp"
+#include "vdk.h"
+
+namespace vdk {
+
+typedef __bf16 bf16_t;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+
+template <class T> struct Vec8;
+template <> struct Vec8<half_t> {
+    using type = half8;
+    using pair = _Float16 __attribute__((ext_vector_type(2)));
+};
+template <> struct Vec8<bf16_t> {
+    using type = bf16x8;
+    using pair = __bf16 __attribute__((ext_vector_type(2)));
+};
+
+// D = A B + C on 32 x 32 x 16: lane l holds row (column) l % 32 of A (B) and
+// k = 8 (l / 32) .. + 7; C / D register r is row 8 (r / 4) + 4 (l / 32) + r % 4
+// of column l % 32.
+__device__ __forceinline__ float16v mfma32(half8 a, half8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16v mfma32(bf16x8 a, bf16x8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even and packed (one v_cvt_pk).
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::pair pack2(float a, float b) {
+    return __builtin_convertvector((float2v{a, b}), typename Vec8<T>::pair);
+}
+
+// Registers 8 c .. 8 c + 7 of a C block as a B operand's eight k-slots: lane
+// half h then holds rows 16 c + 4 h + {0..3} and 16 c + 8 + 4 h + {0..3}, the
+// rows that tr_pair gives it for the A operand.
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type pack8(const float16v& s, int c) {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const auto p = pack2<T>(s[8 * c + j], s[8 * c + j + 1]);
+        v[j] = p[0];
+        v[j + 1] = p[1];
+    }
+    return v;
+}
+
+__device__ __forceinline__ float16v splat16(float x) {
+    float16v v;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = x;
+    return v;
+}
+
+// What pack8 rounded away, rounded itself: the two together hold twice the bits.
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type rest8(const float16v& s, typename Vec8<T>::type hi, int c) {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const auto p = pack2<T>(s[8 * c + j] - (float)hi[j], s[8 * c + j + 1] - (float)hi[j + 1]);
+        v[j] = p[0];
+        v[j + 1] = p[1];
+    }
+    return v;
+}
+
+// The other 32 lanes' value.
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// ---- LDS tiles of D 16-bit columns, dense rows ----
+// Row r's 16-byte chunk c lies at chunk position c ^ swz(r).  Sixteen rows'
+// same chunk (an A operand's read) then lie in sixteen different bank groups,
+// and so do four rows' four neighbouring chunks (a transposing read).
+template <int D>
+__device__ __forceinline__ int tile_swz(int row) {
+    return D == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {   // byte offset
+    return row * (2 * D) + ((chunk ^ tile_swz<D>(row)) << 4);
+}
+
+// ROWS rows from `src` (row stride in bytes, `valid` of them exist, the others
+// read as zero) into an LDS tile by DMA, spread over NW waves.
+template <int D, int ROWS, int NW>
+struct TileDma {
+    static constexpr int kOps = ROWS * D / 512;             // 1 KB each
+    static constexpr int kPer = (kOps + NW - 1) / NW;
+    uint32_t voff[kPer];
+    __device__ __forceinline__ void init(uint32_t row_bytes, int wave, int lane) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = (j * NW + wave) * 64 + lane, row = i / (D / 8), pos = i % (D / 8);
+            voff[j] = row * row_bytes + ((pos ^ tile_swz<D>(row)) << 4);
+        }
+    }
+    __device__ __forceinline__ void load(uint8_t* lds, const void* src, uint32_t row_bytes, int valid, int wave) const {
+        const int n = valid < ROWS ? valid : ROWS;
+        const int4v rsrc = dma_rsrc(src, n > 0 ? (uint32_t)(n - 1) * row_bytes + 2 * D : 0);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (kOps % NW == 0 || j * NW + wave < kOps) dma16(lds + (j * NW + wave) * 1024, rsrc, voff[j]);
+    }
+};
+
+// A operand rows row0 + lane % 32, columns 16 kk + 8 (lane / 32) .. + 7.
+template <class T, int D>
+__device__ __forceinline__ typename Vec8<T>::type tile_rows(const uint8_t* lds, int row0, int kk, int lane) {
+    return *reinterpret_cast<const typename Vec8<T>::type*>(
+        lds + tile_at<D>(row0 + (lane & 31), 2 * kk + (lane >> 5)));
+}
+
+// A operand of the transposed tile: row (of A) = column 32 dt + lane % 32 of
+// the tile, its eight k-slots the tile's rows row0 + 4 h + {0..3} and row0 + 8
+// + 4 h + {0..3} (h = lane / 32).  Of each 16 lanes of a transposing read, lane
+// i supplies 8 bytes of row i / 4 and receives column i of the four rows.
+template <class T, int D>
+__device__ __forceinline__ typename Vec8<T>::type tr_pair(const uint8_t* lds, int row0, int dt, int lane) {
+    const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2);
+    const int col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+    const uint8_t* p0 = lds + tile_at<D>(row, col >> 3) + (col & 4) * 2;
+    const uint8_t* p1 = lds + tile_at<D>(row + 8, col >> 3) + (col & 4) * 2;
+    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p0);
+    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p1);
+    return __builtin_bit_cast(typename Vec8<T>::type, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- scores ----
+// Scores are kept in units of log 2: s2 = am * w + ab + bias2, with w = q . k
+// without a cap.  With one, tanh(y) = 1 - 2 / (1 + exp(2 y)) takes w = -1 / (1 +
+// exp(2 y)): one exp2, one add, one reciprocal.  Its error is that of a 32-bit
+// rounding near 1 (6e-8 cap), so caps above 64 take w = tanh(y) from a series
+// where |y| is small instead.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kWideCap = 64.0f;
+
+struct ScoreMap {
+    float mul, am, ab;   // mul: q . k to the exponent (or y)
+    int wide;
+};
+
+inline ScoreMap score_map(float scale, float cap) {
+    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f, 0};
+    if (cap > kWideCap) return {scale / cap, cap * kLog2e, 0.0f, 1};
+    return {2.0f * kLog2e * scale / cap, 2.0f * cap * kLog2e, cap * kLog2e, 0};
+}
+
+__device__ __forceinline__ float tanh_series(float y) {
+    const float y2 = y * y;
+    const float t = y * (1.0f + y2 * (-1.0f / 3 + y2 * (2.0f / 15 + y2 * (-17.0f / 315 + y2 * (62.0f / 2835)))));
+    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * y);
+    return fabsf(y) < 0.25f ? t : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// q . k of a block to w, in place.
+template <bool CAP>
+__device__ __forceinline__ void score_w(float16v& s, const ScoreMap& m) {
+    if constexpr (CAP) {
+        if (m.wide) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = tanh_series(s[r] * m.mul);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[r] * m.mul));
+        }
+    }
+}
+
+// A bias in units of log 2; finite values stay finite, so that a row of the
+// type's lowest value keeps an even softmax.
+__device__ __forceinline__ float bias2_of(float b) {
+    const float x = b * kLog2e;
+    return fabsf(b) == INFINITY ? b : fminf(fmaxf(x, -FLT_MAX), FLT_MAX);
+}
+
+constexpr int kKeys = 64;     // rows of a step's tiles
+constexpr int kTabPad = 96;   // a tile of 64 x 32 that touches a distance inside (-R, R) reaches 95 past it
+
+// ---- packed layouts ----
+struct AttnClip {
+    long long q0, k0;   // first query and key
+    int nq, nk, prefix;
+    int b32;                // blocks of 32 queries before the clip's
+};
+
+// Argument checks shared by the forward and the backward call.
+void check_rows(const void* p, long long tok, long long head, int dim, const char* name);
+void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a);
+
+}  // namespace vdk
+
+// Work lists hold (clip, first row) of 128 queries or keys, heaviest first.
+struct vdk_attn_plan {
+    int n_clips, n_heads, n_kv, dim, causal;
+    long long total_q, total_kv;
+    std::vector<vdk::AttnClip> clips;
+    int n_q128, n_k128, n_b32;   // (n_b32: blocks of 32 queries)
+    void* device;                  // one allocation for all tables
+    vdk::AttnClip* d_clips;
+    int2 *d_q128, *d_k128;
+};

@@ -1,0 +1,596 @@
+// kvcache.hip - the paged key-value cache of streams: rows written (quantised
+// as they are written) and read back, and one new frame's attention over it.
+#include <algorithm>
+
+#include "attn.hpp"
+
+namespace vdk {
+namespace {
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef int int2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) int2v lds_int2v;
+
+constexpr float kE4m3Max = 448.0f, kTiny = 5.421010862427522e-20f;   // 2^-64
+
+// ---- rows written and read ----
+// One thread holds 16 values of a row (32 bytes in, 16 codes out), D / 16
+// neighbouring lanes a row; keys and values in one launch.  Both directions
+// are bound by memory: a row is read once and written once.
+struct RowArgs {
+    uint8_t *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    const long long* slots;
+    long long n, n_slots;
+    int kv, page, page_shift;
+    void *k, *v;
+    long long k_tok, k_head, v_tok, v_head;
+    int* status;
+};
+
+__device__ __forceinline__ float2v from_e4m3(uint32_t w, int hi) {
+    return hi ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+}
+
+template <class T, int D, bool QUANT, bool WRITE>
+__global__ __launch_bounds__(256) void cache_rows_kernel(RowArgs a) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int kLanes = D / 16, kRow = QUANT ? D : 2 * D;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int c = (int)(i % kLanes);
+    const long long row = i / kLanes, tok = row / a.kv;
+    const int h = (int)(row - tok * a.kv), which = blockIdx.y;
+    if (tok >= a.n) return;                                // whole rows leave together
+    const long long slot = a.slots[tok];
+    const bool ok = slot >= 0 && slot < a.n_slots;
+    if (slot >= a.n_slots && c == 0 && h == 0 && which == 0 && a.status) atomicOr(a.status, VDK_STATUS_BAD_SLOT);
+    if (WRITE && !ok) return;
+    const long long at = (((slot >> a.page_shift) * a.kv + h) << a.page_shift) + (slot & (a.page - 1));
+    uint8_t* held = (which ? a.v_cache : a.k_cache) + at * kRow;
+    float* scale = which ? a.v_scale : a.k_scale;
+    T* x = static_cast<T*>(which ? a.v : a.k) + tok * (which ? a.v_tok : a.k_tok) + h * (which ? a.v_head : a.k_head) +
+           16 * c;
+    if constexpr (WRITE) {
+        V8 v[2];
+        v[0] = *reinterpret_cast<const V8*>(x);
+        v[1] = *reinterpret_cast<const V8*>(x + 8);
+        if constexpr (!QUANT) {
+            *reinterpret_cast<V8*>(held + 32 * c) = v[0];
+            *reinterpret_cast<V8*>(held + 32 * c + 16) = v[1];
+        } else {
+            float f[16], most = kTiny;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                f[j] = (float)v[j >> 3][j & 7];
+                most = fmaxf(most, fabsf(f[j]));
+                bad |= !(fabsf(f[j]) <= FLT_MAX);
+            }
+            if (bad) most = INFINITY;
+#pragma unroll
+            for (int off = 1; off < kLanes; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+            bad = most == INFINITY;
+            // the quotient 448 x / most, rounded once: an approximate one and its exact remainder.  A quotient that is a
+            // tie between two codes has few bits, so it comes out exact, and 16-bit x leave none nearer than 2^-17 to one.
+            const float inv = __builtin_amdgcn_rcpf(most);
+            float y[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float t = f[j] * kE4m3Max, q = t * inv;
+                y[j] = bad ? 0.0f : __builtin_fmaf(__builtin_fmaf(-q, most, t), inv, q);
+            }
+            int4v w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                int u = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j], y[4 * j + 1], 0, false);
+                w[j] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j + 2], y[4 * j + 3], u, true);
+            }
+            *reinterpret_cast<int4v*>(held + 16 * c) = w;
+            if (c == 0) scale[at] = bad ? NAN : most / kE4m3Max;
+        }
+    } else {
+        V8 v[2];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j >> 3][j & 7] = (T)0.0f;
+        if (ok) {
+            if constexpr (!QUANT) {
+                v[0] = *reinterpret_cast<const V8*>(held + 32 * c);
+                v[1] = *reinterpret_cast<const V8*>(held + 32 * c + 16);
+            } else {
+                const int4v w = *reinterpret_cast<const int4v*>(held + 16 * c);
+                const float s = scale[at];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2v f = from_e4m3(w[j >> 1], j & 1);
+                    const auto p = pack2<T>(f[0] * s, f[1] * s);
+                    v[j >> 2][2 * (j & 3)] = p[0];
+                    v[j >> 2][2 * (j & 3) + 1] = p[1];
+                }
+            }
+        }
+        *reinterpret_cast<V8*>(x) = v[0];
+        *reinterpret_cast<V8*>(x + 8) = v[1];
+    }
+}
+
+// ---- one query a stream ----
+// A workgroup serves up to 16 query heads of one key head over one part of a
+// stream's keys; its 4 waves take 32-key steps in turn, each with its own
+// running maximum, sum and output, joined through LDS at the end.  Keys, values
+// and scales come by DMA into a ring private to the wave, so no barrier stands
+// in the loop.  Per step, on MFMA 16x16x32: S (keys x heads) = K Q^T, then
+// O^T (dims x heads) += V^T P^T, V^T by transposing LDS loads; e4m3 codes
+// become 16-bit values exactly on their way from LDS.  The scale of a key
+// multiplies its score, that of a value its p.
+constexpr int kStep = 32, kWaves = 4;
+
+struct PagedArgs {
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    int n_pages, page_shift, kv;
+    const void* q;
+    long long q_seq, q_head;
+    const int *table, *lens;
+    int max_pages, max_len, n_heads, group, head_parts, splits, chunk;
+    const float* bias;
+    int radius;
+    ScoreMap map;
+    void* o;
+    long long o_seq, o_head;
+    float *lse, *part;
+    int* status;
+};
+
+__device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float4v mfma16(bf16x8 a, bf16x8 b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Eight e4m3 codes as 16-bit values (exact: 4 significant bits, 2^-9 .. 448).
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type codes8(uint32_t lo, uint32_t hi) {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2v f = from_e4m3(j < 2 ? lo : hi, j & 1);
+        const auto p = pack2<T>(f[0], f[1]);
+        v[2 * j] = p[0];
+        v[2 * j + 1] = p[1];
+    }
+    return v;
+}
+
+// DMA of BYTES a lane from per-lane addresses to LDS lds_dst + BYTES * lane
+// (lds_dst wave-uniform); ordered by the caller's vmcnt waits.
+template <int BYTES>
+__device__ __forceinline__ void dma_lanes(uint8_t* lds_dst, const void* src) {
+    const uint32_t m0v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)lds_dst);
+    if constexpr (BYTES == 16)
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
+    else
+        asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
+}
+
+// 16-byte chunk c of ring row r: rows of RB bytes, swizzled so that the column
+// of 16-byte pieces that a transposing read takes spreads over all banks.
+template <int RB>
+__device__ __forceinline__ int ring_chunk(int row, int c) {
+    return RB == 64 ? c ^ ((row >> 2) & 3) : RB == 128 ? c ^ ((row >> 1) & 7) : c ^ (row & 15);
+}
+
+template <class T, int D, bool QUANT>
+struct PagedShape {
+    static constexpr int kRow = QUANT ? D : 2 * D;
+    static constexpr int kTile = kStep * kRow;                       // keys (or values) of a step
+    static constexpr int kStage = 2 * kTile + (QUANT ? 256 : 0);     // + 32 + 32 scales
+    static constexpr int kOps = 2 * kTile / 1024 + (QUANT ? 1 : 0);  // DMA instructions of a stage
+    static constexpr int kDepth = kTile <= 4096 ? 3 : 2;
+    static constexpr int kRing = kWaves * kDepth * kStage;
+    static constexpr int kJoin = kWaves * 16 * (D + 4) * 4;          // after the loop, in the ring's place
+    static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+};
+
+template <class T, int D, bool QUANT, bool CAP>
+__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
+    using S = PagedShape<T, D, QUANT>;
+    using V8 = typename Vec8<T>::type;
+    using PT = std::conditional_t<QUANT, bf16_t, T>;   // p times a value's scale may leave the range of f16
+    using P8 = typename Vec8<PT>::type;
+    constexpr int kRow = S::kRow, kChunks = kRow / 16;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    int* pages = reinterpret_cast<int*>(smem + S::kLds);
+    const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits, part = rest % a.head_parts,
+              rest2 = rest / a.head_parts, kvh = rest2 % a.kv, seq = rest2 / a.kv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n16 = lane & 15,
+              g = lane >> 4;
+    const int page = 1 << a.page_shift;
+    const int want = a.lens[seq], len = min(max(want, 0), a.max_len);
+    if (want != len && split == 0 && kvh == 0 && part == 0 && threadIdx.x == 0 && a.status)
+        atomicOr(a.status, VDK_STATUS_BAD_LENGTH);
+    const int k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
+    if (k0 >= k1 && split > 0) return;
+    // the part's pages; -1 for one outside the cache
+    const int p0 = k0 >> a.page_shift, np = k1 > k0 ? ((k1 - 1) >> a.page_shift) - p0 + 1 : 0;
+    for (int i = threadIdx.x; i < np; i += 64 * kWaves) {
+        int p = a.table[(long long)seq * a.max_pages + p0 + i];
+        if (p < 0 || p >= a.n_pages) {
+            p = -1;
+            if (a.status) atomicOr(a.status, VDK_STATUS_BAD_PAGE);
+        }
+        pages[i] = p;
+    }
+    const int hq = part * 16 + n16, head = kvh * a.group + min(hq, a.group - 1);
+    const T* qp = static_cast<const T*>(a.q) + seq * a.q_seq + head * a.q_head;
+    V8 qf[D / 32];   // slot (g, j) of product kk: e4m3 dims 64 (kk / 2) + 16 g + 8 (kk % 2) + j, else 32 kk + 8 g + j
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk)
+        qf[kk] = *reinterpret_cast<const V8*>(qp + (QUANT ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
+    const float* bias = a.bias ? a.bias + (long long)head * (2 * a.radius + 1) : nullptr;
+    __syncthreads();
+
+    uint8_t* ring = smem + wave * S::kDepth * S::kStage;
+    auto row_of = [&](int key) {   // the cache row of a key (clamped into the part), its page -1: row 0 (hidden later)
+        const int k = min(key, k1 - 1), p = max(pages[(k >> a.page_shift) - p0], 0);
+        return (((long long)p * a.kv + kvh) << a.page_shift) + (k & (page - 1));
+    };
+    auto fetch = [&](int kb, int st) {
+        uint8_t* dst = ring + st * S::kStage;
+#pragma unroll
+        for (int j = 0; j < S::kTile / 1024; ++j) {
+            const int i = j * 64 + lane, r = i / kChunks, c = ring_chunk<kRow>(r, i % kChunks);
+            const long long at = row_of(kb + r) * kRow + 16 * c;
+            dma_lanes<16>(dst + j * 1024, a.k + at);
+            dma_lanes<16>(dst + S::kTile + j * 1024, a.v + at);
+        }
+        if constexpr (QUANT)   // lanes 0..31: the keys' scales, 32..63: the values'
+            dma_lanes<4>(dst + 2 * S::kTile, (lane < 32 ? a.k_scale : a.v_scale) + row_of(kb + (lane & 31)));
+    };
+    const int first = k0 + wave * kStep;
+    const int steps = first < k1 ? (k1 - first + kWaves * kStep - 1) / (kWaves * kStep) : 0;
+#pragma unroll
+    for (int st = 0; st < S::kDepth - 1; ++st)
+        if (st < steps) fetch(first + st * kWaves * kStep, st);
+
+    float4v o[D / 16];
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[dt] = float4v{0, 0, 0, 0};
+    float m = -FLT_MAX, l = 0.0f;
+    int st = 0;
+    for (int it = 0; it < steps; ++it, st = st + 1 == S::kDepth ? 0 : st + 1) {
+        const int kb = first + it * kWaves * kStep;
+        __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the stage to be filled is no longer read
+        if (it + S::kDepth - 1 < steps) {
+            fetch(kb + (S::kDepth - 1) * kWaves * kStep, st == 0 ? S::kDepth - 1 : st - 1);
+            wait_vmcnt<(S::kDepth - 1) * S::kOps>();
+        } else {
+            wait_vmcnt<0>();
+        }
+        asm volatile("" ::: "memory");
+        const uint8_t* sk = ring + st * S::kStage;
+        const uint8_t* sv = sk + S::kTile;
+        const float* sc = reinterpret_cast<const float*>(sk + 2 * S::kTile);
+        // s[t][r]: key kb + 16 t + 4 g + r, head n16
+        float4v s[2];
+        float mx = -INFINITY;
+        bool there[2];   // whether the 16 keys' page exists
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = float4v{0, 0, 0, 0};
+            const int row = 16 * t + n16;
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const int4v w = *reinterpret_cast<const int4v*>(sk + row * kRow + 16 * ring_chunk<kRow>(row, 4 * i + g));
+                    s[t] = mfma16(codes8<T>(w[0], w[1]), qf[2 * i], s[t]);
+                    s[t] = mfma16(codes8<T>(w[2], w[3]), qf[2 * i + 1], s[t]);
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < D / 32; ++kk)
+                    s[t] = mfma16(*reinterpret_cast<const V8*>(sk + row * kRow + 16 * ring_chunk<kRow>(row, 4 * kk + g)),
+                                  qf[kk], s[t]);
+            }
+            const int kt = kb + 16 * t + 4 * g;
+            there[t] = pages[(min(kb + 16 * t, k1 - 1) >> a.page_shift) - p0] >= 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float w = s[t][r];
+                if constexpr (QUANT) w *= sc[16 * t + 4 * g + r];
+                if constexpr (CAP)
+                    w = a.map.wide ? tanh_series(w * a.map.mul)
+                                   : __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(w * a.map.mul));
+                const int d = min(max(kt + r - (len - 1), -a.radius), 0) + a.radius;   // (keys past the last: hidden)
+                const float b2 = bias ? bias2_of(bias[d]) : 0.0f;
+                w = __builtin_fmaf(w, a.map.am, a.map.ab + b2);
+                s[t][r] = there[t] && kt + r < k1 ? w : -INFINITY;
+                mx = fmaxf(mx, s[t][r]);
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__any(mx > m + 8.0f)) {
+            const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) o[dt] *= float4v{alpha, alpha, alpha, alpha};
+        }
+        P8 hi, lo;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float p = __builtin_amdgcn_exp2f(s[t][r] - m);
+                l += p;
+                if constexpr (QUANT) p = s[t][r] == -INFINITY ? 0.0f : p * sc[32 + 16 * t + 4 * g + r];
+                hi[4 * t + r] = (PT)p;
+                // half type: p in two bf16 parts, 16 bits of it together
+                if constexpr (QUANT) lo[4 * t + r] = (PT)(p - (float)hi[4 * t + r]);
+            }
+        // V^T: row (dim) n16 of tile dt, slots the keys 4 g + {0..3} and 16 + 4 g + {0..3}
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            if constexpr (QUANT) {
+                const int j = n16 >> 1, row = 16 * (j >> 2) + 4 * g + (j & 3);
+                const uint8_t* p = sv + row * kRow + 16 * ring_chunk<kRow>(row, dt) + 8 * (n16 & 1);
+                const int2v w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2v*)p);
+                const P8 va = codes8<PT>(there[0] ? w[0] : 0, there[1] ? w[1] : 0);
+                o[dt] = mfma16(va, hi, o[dt]);
+                if constexpr (std::is_same_v<T, half_t>) o[dt] = mfma16(va, lo, o[dt]);
+            } else {
+                const int r0 = 4 * g + (n16 >> 2), r1 = 16 + r0, c = 2 * dt + ((n16 & 3) >> 1), e = 8 * (n16 & 1);
+                const short4v x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_short4v*)(sv + r0 * kRow + 16 * ring_chunk<kRow>(r0, c) + e));
+                const short4v x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_short4v*)(sv + r1 * kRow + 16 * ring_chunk<kRow>(r1, c) + e));
+                const short4v none = {0, 0, 0, 0}, y0 = there[0] ? x0 : none, y1 = there[1] ? x1 : none;
+                o[dt] = mfma16(__builtin_bit_cast(P8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7)), hi, o[dt]);
+            }
+        }
+    }
+    // join the waves: [wave][head][D + 4] with the maximum and the sum behind the D values
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();
+    constexpr int kJ = D + 4;
+    float* js = reinterpret_cast<float*>(smem);
+    float* mine = js + (wave * 16 + n16) * kJ;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4v*>(mine + 16 * dt + 4 * g) = o[dt];
+    if (g == 0) {
+        mine[D] = m;
+        mine[D + 1] = l;
+    }
+    __syncthreads();
+    const int heads = min(a.group - part * 16, 16);
+    for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kWaves) {
+        const int hh = i / (D / 4), d = 4 * (i % (D / 4));
+        const float* p = js + hh * kJ;
+        float mm = -FLT_MAX;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, p[w * 16 * kJ + D]);
+        float ll = 0.0f;
+        float4v v = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(p[w * 16 * kJ + D] - mm);
+            ll += f * p[w * 16 * kJ + D + 1];
+            v += float4v{f, f, f, f} * *reinterpret_cast<const float4v*>(p + w * 16 * kJ + d);
+        }
+        const int hd = kvh * a.group + part * 16 + hh;
+        const long long row = (long long)seq * a.n_heads + hd;
+        if (a.splits > 1) {
+            float* out = a.part + (row * a.splits + split) * kJ;
+            *reinterpret_cast<float4v*>(out + d) = v;
+            if (d == 0) {
+                out[D] = mm;
+                out[D + 1] = ll;
+            }
+        } else {
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            T* op = static_cast<T*>(a.o) + seq * a.o_seq + hd * a.o_head + d;
+            const auto u0 = pack2<T>(v[0] * inv, v[1] * inv), u1 = pack2<T>(v[2] * inv, v[3] * inv);
+            *reinterpret_cast<uint2*>(op) = uint2{__builtin_bit_cast(uint32_t, u0), __builtin_bit_cast(uint32_t, u1)};
+            if (d == 0 && a.lse)
+                a.lse[row] = ll == 0.0f ? -INFINITY
+                             : mm > -FLT_MAX ? (mm + __builtin_amdgcn_logf(ll)) * 0.69314718055994531f
+                                             : -FLT_MAX;
+        }
+    }
+}
+
+// The parts of one (stream, head), one wave each: the exponents' common maximum, then the weighted sum.
+template <class T, int D>
+__global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs a) {
+    constexpr int kJ = D + 4, kPer = D / 64;
+    const long long row = blockIdx.x;
+    const int seq = (int)(row / a.n_heads), head = (int)(row % a.n_heads), lane = threadIdx.x;
+    const int len = min(max(a.lens[seq], 0), a.max_len), n = max((len + a.chunk - 1) / a.chunk, 1);
+    const float* p = a.part + row * a.splits * kJ;
+    float m = -FLT_MAX;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, p[i * kJ + D]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    float l = 0.0f, v[kPer] = {};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float f = __builtin_amdgcn_exp2f(p[i * kJ + D] - m);
+        l += f * p[i * kJ + D + 1];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[e] += f * p[i * kJ + kPer * lane + e];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* op = static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) op[e] = (T)(v[e] * inv);
+    if (lane == 0 && a.lse)
+        a.lse[row] = l == 0.0f ? -INFINITY
+                     : m > -FLT_MAX ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
+                                    : -FLT_MAX;
+}
+
+void check_cache(const vdk_kv_cache* c, const std::string& w) {
+    require(c, w + ": NULL cache");
+    require(c->dtype == VDK_F16 || c->dtype == VDK_BF16, w + ": dtype must be VDK_F16 or VDK_BF16");
+    require(c->format == VDK_KV_16 || c->format == VDK_KV_E4M3, w + ": format must be VDK_KV_16 or VDK_KV_E4M3");
+    require(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
+            w + ": page_size must be 16, 32, 64 or 128");
+    require(c->head_dim == 64 || c->head_dim == 128, w + ": head_dim must be 64 or 128");
+    require(c->n_pages > 0 && c->n_kv_heads > 0 && c->n_kv_heads <= 1024, w + ": empty cache or too many heads");
+    require(c->k && c->v && (c->format == VDK_KV_16 || (c->k_scale && c->v_scale)), w + ": NULL cache pointer");
+    require((uintptr_t)c->k % 16 == 0 && (uintptr_t)c->v % 16 == 0 && (uintptr_t)c->k_scale % 16 == 0 &&
+                (uintptr_t)c->v_scale % 16 == 0,
+            w + ": cache pointers must be 16-byte aligned");
+}
+
+void check_strided(const void* p, long long a, long long b, const std::string& w) {
+    require(p, w + " is NULL");
+    require((uintptr_t)p % 16 == 0 && a % 8 == 0 && b % 8 == 0 && a >= 0 && b >= 0,
+            w + ": 16-byte aligned pointer and strides of multiples of 8, please");
+}
+
+int shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+template <bool WRITE>
+int cache_rows(const vdk_kv_cache* c, const long long* slots, long long n, void* k, long long k_tok, long long k_head,
+               void* v, long long v_tok, long long v_head, int* status, void* stream, const char* what) {
+    return guarded([&] {
+        const std::string w(what);
+        check_cache(c, w);
+        require(n >= 0, w + ": negative number of tokens");
+        if (n == 0) return;
+        require(slots && (uintptr_t)slots % 8 == 0 && (uintptr_t)status % 4 == 0, w + ": NULL or misaligned slots");
+        check_strided(k, k_tok, k_head, w + ": k");
+        check_strided(v, v_tok, v_head, w + ": v");
+        const long long threads = n * c->n_kv_heads * (c->head_dim / 16);
+        require(n <= (1ll << 40) / c->n_kv_heads && threads <= (1ll << 38), w + ": too many tokens for one launch");
+        RowArgs a{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, slots, n,
+                  (long long)c->n_pages * c->page_size, c->n_kv_heads, c->page_size, shift_of(c->page_size), k, v,
+                  k_tok, k_head, v_tok, v_head, status};
+        const dim3 grid((unsigned)((threads + 255) / 256), 2);
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a); };
+        const bool q = c->format == VDK_KV_E4M3, d64 = c->head_dim == 64;
+        if (c->dtype == VDK_F16)
+            d64 ? (q ? go(cache_rows_kernel<half_t, 64, true, WRITE>) : go(cache_rows_kernel<half_t, 64, false, WRITE>))
+                : (q ? go(cache_rows_kernel<half_t, 128, true, WRITE>) : go(cache_rows_kernel<half_t, 128, false, WRITE>));
+        else
+            d64 ? (q ? go(cache_rows_kernel<bf16_t, 64, true, WRITE>) : go(cache_rows_kernel<bf16_t, 64, false, WRITE>))
+                : (q ? go(cache_rows_kernel<bf16_t, 128, true, WRITE>) : go(cache_rows_kernel<bf16_t, 128, false, WRITE>));
+        VDK_HIP(hipGetLastError());
+    });
+}
+
+// How many parts a stream's keys are cut into, and how long one is.
+struct Cut {
+    int splits, chunk;
+};
+Cut cut_of(const vdk_kv_cache* c, const vdk_paged_attn* a) {
+    const long long groups = (long long)a->n_seqs * c->n_kv_heads * cdiv(a->n_q_heads / c->n_kv_heads, 16);
+    const long long want = std::max(1ll, 2048 / std::max(groups, 1ll));
+    long long chunk = (a->max_len + want - 1) / want;
+    chunk = std::min(std::max((chunk + 127) / 128 * 128, 512ll), 8192ll);
+    return {(int)std::max(1ll, (a->max_len + chunk - 1) / chunk), (int)chunk};
+}
+
+void check_paged(const vdk_kv_cache* c, const vdk_paged_attn* a) {
+    const std::string w("paged_attention");
+    check_cache(c, w);
+    require(a, w + ": NULL description");
+    require(a->n_seqs >= 0 && a->max_pages >= 0 && a->max_len >= 0, w + ": negative size");
+    require(a->n_q_heads > 0 && a->n_q_heads % c->n_kv_heads == 0 && a->n_q_heads <= 1024,
+            w + ": n_q_heads must be a multiple of n_kv_heads, at most 1024");
+    require(a->max_len <= (long long)a->max_pages * c->page_size, w + ": max_len exceeds the block table");
+    require(a->max_len <= (1 << 30), w + ": max_len must be 2^30 at most");
+}
+
+template <class T, int D, bool QUANT, bool CAP>
+void launch_paged(PagedArgs a, int n_seqs, hipStream_t s) {
+    auto kern = paged_attn_kernel<T, D, QUANT, CAP>;
+    const int lds = PagedShape<T, D, QUANT>::kLds + 4 * ((a.chunk >> a.page_shift) + 2);
+    if (lds > 65536)
+        VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(kern, dim3((unsigned)n_seqs * a.kv * a.head_parts * a.splits), dim3(64 * kWaves), lds, s, a);
+    VDK_HIP(hipGetLastError());
+    if (a.splits > 1) {
+        hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)n_seqs * a.n_heads), dim3(64), 0, s, a);
+        VDK_HIP(hipGetLastError());
+    }
+}
+
+template <class T, int D>
+void launch_paged_f(const PagedArgs& a, int n_seqs, bool quant, bool cap, hipStream_t s) {
+    if (quant) cap ? launch_paged<T, D, true, true>(a, n_seqs, s) : launch_paged<T, D, true, false>(a, n_seqs, s);
+    else cap ? launch_paged<T, D, false, true>(a, n_seqs, s) : launch_paged<T, D, false, false>(a, n_seqs, s);
+}
+
+}  // namespace
+}  // namespace vdk
+
+using namespace vdk;
+
+extern "C" int vdk_kv_cache_write(const vdk_kv_cache* c, const long long* d_slots, long long n, const void* d_k,
+                                  long long k_tok, long long k_head, const void* d_v, long long v_tok,
+                                  long long v_head, int* d_status, void* stream) {
+    return cache_rows<true>(c, d_slots, n, const_cast<void*>(d_k), k_tok, k_head, const_cast<void*>(d_v), v_tok, v_head,
+                            d_status, stream, "kv_cache_write");
+}
+
+extern "C" int vdk_kv_cache_read(const vdk_kv_cache* c, const long long* d_slots, long long n, void* d_k,
+                                 long long k_tok, long long k_head, void* d_v, long long v_tok, long long v_head,
+                                 int* d_status, void* stream) {
+    return cache_rows<false>(c, d_slots, n, d_k, k_tok, k_head, d_v, v_tok, v_head, d_status, stream, "kv_cache_read");
+}
+
+extern "C" size_t vdk_paged_attention_workspace_size(const vdk_kv_cache* c, const vdk_paged_attn* a) {
+    size_t n = 0;
+    if (guarded([&] {
+            check_paged(c, a);
+            const Cut cut = cut_of(c, a);
+            if (cut.splits > 1) n = (size_t)a->n_seqs * a->n_q_heads * cut.splits * (c->head_dim + 4) * 4;
+        }) != 0)
+        return 0;
+    return n;
+}
+
+extern "C" int vdk_paged_attention(const vdk_kv_cache* c, const vdk_paged_attn* a, void* stream) {
+    return guarded([&] {
+        const std::string w("paged_attention");
+        check_paged(c, a);
+        require(std::isfinite(a->scale) && a->scale > 0.0f, w + ": scale must be positive and finite");
+        require(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
+                w + ": cap must be 0 or 1e-3 .. 1e6");
+        require(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= 4096), w + ": bias_radius must be 1 .. 4096");
+        if (a->n_seqs == 0) return;
+        require(a->seq_lens && (a->block_table || a->max_len == 0), w + ": NULL table or lengths");
+        require((uintptr_t)a->seq_lens % 4 == 0 && (uintptr_t)a->block_table % 4 == 0 && (uintptr_t)a->dist_bias % 4 == 0 &&
+                    (uintptr_t)a->lse % 4 == 0 && (uintptr_t)a->status % 4 == 0,
+                w + ": misaligned pointer");
+        check_strided(a->q, a->q_seq, a->q_head, w + ": q");
+        check_strided(a->o, a->o_seq, a->o_head, w + ": o");
+        const Cut cut = cut_of(c, a);
+        const int group = a->n_q_heads / c->n_kv_heads, parts = cdiv(group, 16);
+        if (cut.splits > 1) {
+            const size_t need = vdk_paged_attention_workspace_size(c, a);
+            require(a->work && a->work_bytes >= need && (uintptr_t)a->work % 16 == 0,
+                    w + ": workspace missing, misaligned or smaller than vdk_paged_attention_workspace_size");
+        }
+        require((long long)a->n_seqs * c->n_kv_heads * parts * cut.splits < (1ll << 31) &&
+                    (long long)a->n_seqs * a->n_q_heads < (1ll << 31),
+                w + ": too many streams for one launch");
+        PagedArgs p{static_cast<const uint8_t*>(c->k), static_cast<const uint8_t*>(c->v), c->k_scale, c->v_scale,
+                    c->n_pages, shift_of(c->page_size), c->n_kv_heads, a->q, a->q_seq, a->q_head, a->block_table,
+                    a->seq_lens, a->max_pages, a->max_len, a->n_q_heads, group, parts, cut.splits, cut.chunk,
+                    a->dist_bias, a->dist_bias ? a->bias_radius : 0, score_map(a->scale, a->cap), a->o, a->o_seq,
+                    a->o_head, a->lse, static_cast<float*>(a->work), a->status};
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        const bool q = c->format == VDK_KV_E4M3, cap = a->cap > 0;
+        if (c->dtype == VDK_F16)
+            c->head_dim == 64 ? launch_paged_f<half_t, 64>(p, a->n_seqs, q, cap, s)
+                              : launch_paged_f<half_t, 128>(p, a->n_seqs, q, cap, s);
+        else
+            c->head_dim == 64 ? launch_paged_f<bf16_t, 64>(p, a->n_seqs, q, cap, s)
+                              : launch_paged_f<bf16_t, 128>(p, a->n_seqs, q, cap, s);
+    });
+}

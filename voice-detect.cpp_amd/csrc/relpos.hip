@@ -1,0 +1,432 @@
+// relpos.hip - attention with a learned position bias over packed clips, the
+// plan of their layout, and the bias of each distance from a table of buckets.
+#include <algorithm>
+
+#include "attn.hpp"
+
+namespace vdk {
+namespace {
+
+constexpr int kMaxRadius = 4096;
+
+struct FwdArgs {
+    const void *q, *k, *v;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    const float* bias;
+    int radius;
+    ScoreMap map;
+    void* o;
+    long long o_tok, o_head;
+    float *o32, *lse;
+    const AttnClip* clips;
+    const int2* tiles;
+    int n_tiles, n_heads, group, causal;
+    long long total_q;
+};
+
+// One workgroup: 32 NW queries of one head, wave w its rows 32 w ..; 64 keys a
+// step through double-buffered LDS tiles.  S^T = K Q^T leaves a query's scores
+// in one lane (pair), so the softmax needs no exchange inside the loop: the
+// row's running maximum moves only when it grows by more than 8 (p <= 2^8, and
+// 16-bit p keep their relative precision), and each lane sums its own keys.
+// P^T then is the B operand of O^T += V^T P^T, V^T read by transposing LDS loads.
+// SPLIT (training, where o_f32 is wanted): P enters in two 16-bit parts, since
+// the backward pass takes delta = sum(o dO) from o, and a bias's gradient sums
+// dS over many rows, where errors of 2^-9 in P would show in a 32-bit result.
+template <class T, int D, int NW, bool CAP, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int kTile = kKeys * D * 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
+    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int h = id / a.n_tiles;
+    const int2 tile = a.tiles[id - h * a.n_tiles];
+    const AttnClip c = a.clips[tile.x];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
+              hl = lane >> 5;
+    const int past = c.nk - c.nq, qw = tile.y + 32 * wave, qi = qw + lr;
+    const int qr = qi < c.nq ? qi : c.nq - 1;
+
+    // keys: [0, kend) for the workgroup, [0, kend_w) for the wave, [0, lim) for the lane's query
+    auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
+    const int kend = max(last(min(tile.y + 32 * NW, c.nq) - 1), 0);
+    const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
+    const int kfull = qw < c.nq ? last(qw) : 0;      // all 32 rows see the keys below
+    const int lim = last(qr);
+
+    const uint32_t kb_row = (uint32_t)a.k_tok * 2, vb_row = (uint32_t)a.v_tok * 2;
+    const T* kp = static_cast<const T*>(a.k) + c.k0 * a.k_tok + (long long)(h / a.group) * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + c.k0 * a.v_tok + (long long)(h / a.group) * a.v_head;
+    TileDma<D, kKeys, NW> dk, dv;
+    dk.init(kb_row, wave, lane);
+    dv.init(vb_row, wave, lane);
+    auto fetch = [&](int kb, int buf) {
+        dk.load(smem + buf * 2 * kTile, kp + (long long)kb * a.k_tok, kb_row, c.nk - kb, wave);
+        dv.load(smem + buf * 2 * kTile + kTile, vp + (long long)kb * a.v_tok, vb_row, c.nk - kb, wave);
+    };
+    if (kend > 0) fetch(0, 0);
+
+    const T* qp = static_cast<const T*>(a.q) + (c.q0 + qr) * a.q_tok + (long long)h * a.q_head;
+    V8 qf[D / 16];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const V8*>(qp + 16 * kk + 8 * hl);
+    const int R = a.radius;
+    float far_l = a.map.ab, far_r = a.map.ab;
+    if (R) {
+        const float* b = a.bias + (long long)h * (2 * R + 1);
+        for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]) + a.map.ab;
+        far_l += bias2_of(b[0]);
+        far_r += bias2_of(b[2 * R]);
+    }
+
+    float16v o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = splat16(0.0f);
+    float m = -FLT_MAX, l = 0.0f;
+    const float am = a.map.am;
+    for (int kb = 0, buf = 0; kb < kend; kb += kKeys, buf ^= 1) {
+        wait_vmcnt<0>();
+        lds_barrier();   // this tile is there, and the other buffer is no longer read
+        if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
+        if (kb >= kend_w) continue;
+        const uint8_t* sk = smem + buf * 2 * kTile;
+        const uint8_t* sv = sk + kTile;
+        float16v s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            s[kt] = splat16(0.0f);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) s[kt] = mfma32(tile_rows<T, D>(sk, 32 * kt, kk, lane), qf[kk], s[kt]);
+            score_w<CAP>(s[kt], a.map);
+        }
+        // s[kt][r]: key kb + 32 kt + 8 (r / 4) + 4 hl + r % 4 of query qi
+        if (kb + kKeys > kfull) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (kb + 32 * kt + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) s[kt][r] = -INFINITY;
+        }
+        const int d0 = kb - (qw + past);   // distances of the tile: d0 - 31 .. d0 + 63
+        const bool near = R != 0 && d0 + 63 > -R && d0 - 31 < R;
+        float mul = am, add = d0 < 0 ? far_l : far_r;
+        if (near) {
+            const float* t = tab + (d0 - lr + 4 * hl + R + kTabPad);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[kt][r] = __builtin_fmaf(s[kt][r], am, t[32 * kt + 8 * (r >> 2) + (r & 3)]);
+            mul = 1.0f;
+            add = 0.0f;
+        } else if (add < -1e37f) {   // a far bias of the lowest value takes the products in, as the near ones do
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_fmaf(s[kt][r], am, add);
+            mul = 1.0f;
+            add = 0.0f;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        mx = __builtin_fmaf(fmaxf(mx, other_half(mx)), mul, add);
+        if (__any(mx > m + 8.0f)) {
+            const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+        }
+        add -= m;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], mul, add));
+                s[kt][r] = p;
+                l += p;
+            }
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+            const V8 pb = pack8<T>(s[cc >> 1], cc & 1);
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) {
+                const V8 vt = tr_pair<T, D>(sv, 16 * cc, dt, lane);
+                o[dt] = mfma32(vt, pb, o[dt]);
+                if constexpr (SPLIT) o[dt] = mfma32(vt, rest8<T>(s[cc >> 1], pb, cc & 1), o[dt]);
+            }
+        }
+    }
+    if (qi >= c.nq) return;
+    l += other_half(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* op = static_cast<T*>(a.o) + (c.q0 + qi) * a.o_tok + (long long)h * a.o_head;
+    float* fp = a.o32 ? a.o32 + ((c.q0 + qi) * a.n_heads + h) * D : nullptr;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float4v v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = o[dt][4 * g + e] * inv;
+            const auto lo = pack2<T>(v[0], v[1]), hi = pack2<T>(v[2], v[3]);
+            const int d = 32 * dt + 8 * g + 4 * hl;
+            uint2 u;
+            u.x = __builtin_bit_cast(uint32_t, lo);
+            u.y = __builtin_bit_cast(uint32_t, hi);
+            *reinterpret_cast<uint2*>(op + d) = u;
+            if (fp) *reinterpret_cast<float4v*>(fp + d) = v;
+        }
+    if (a.lse && hl == 0) {
+        // (a row of the lowest value only: the value itself, its sum lies far below the last bit)
+        const float v = m > -FLT_MAX ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -FLT_MAX;
+        a.lse[h * a.total_q + c.q0 + qi] = l == 0.0f ? -INFINITY : v;
+    }
+}
+
+// ---- the bias by distance from buckets ----
+constexpr int kMaxHalf = 512;
+struct Buckets {
+    int first[kMaxHalf];   // the smallest distance of each bucket of one half
+    int half, both;
+};
+
+Buckets buckets_of(int n_buckets, int bidirectional, int max_distance) {
+    Buckets b;
+    b.both = bidirectional;
+    b.half = bidirectional ? n_buckets / 2 : n_buckets;
+    const int near = b.half / 2;
+    const double per = (b.half - near) / std::log((double)max_distance / near);
+    auto wide = [&](long d) { return near + (long)std::floor(std::log((double)d / near) * per + 1e-9); };
+    for (int i = 0; i < b.half; ++i) {
+        if (i <= near) {
+            b.first[i] = i;
+            continue;
+        }
+        long d = std::max<long>(near, (long)(near * std::exp((i - near) / per)) - 2);
+        while (wide(d) < i) ++d;
+        b.first[i] = (int)std::min<long>(d, INT32_MAX);
+    }
+    return b;
+}
+
+// One thread a distance: its bucket by bisection, then all heads.
+__global__ __launch_bounds__(256) void rel_bias_expand_kernel(const float* __restrict__ table, Buckets b, int heads,
+                                                              int R, float* __restrict__ dist) {
+    __shared__ int first[kMaxHalf];
+    for (int i = threadIdx.x; i < b.half; i += 256) first[i] = b.first[i];
+    __syncthreads();
+    const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (i > 2 * R) return;
+    const int r = i - R;
+    int d = b.both ? abs(r) : max(-r, 0), lo = 0, hi = b.half;   // first[lo] <= d < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= d) lo = mid;
+        else hi = mid;
+    }
+    if (b.both && r > 0) lo += b.half;
+    dist[(long long)h * (2 * R + 1) + i] = table[(long long)lo * heads + h];
+}
+
+// One wave a bucket and head: its distances are one range.
+__global__ __launch_bounds__(64) void rel_bias_reduce_kernel(const float* __restrict__ dist, Buckets b, int heads,
+                                                             int R, float* __restrict__ table) {
+    const int bucket = blockIdx.x, h = blockIdx.y, after = b.both && bucket >= b.half;
+    const int i = after ? bucket - b.half : bucket;
+    int lo = b.first[i], hi = i + 1 < b.half ? b.first[i + 1] - 1 : R;   // distances lo .. hi
+    hi = min(hi, R);
+    int from = after ? max(lo, 1) : -hi, to = after ? hi : -lo;
+    if (!b.both && i == 0) to = R;
+    double sum = 0.0;
+    for (int r = from + (int)threadIdx.x; r <= to; r += 64) sum += dist[(long long)h * (2 * R + 1) + r + R];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (threadIdx.x == 0) table[(long long)bucket * heads + h] = (float)sum;
+}
+
+void check_buckets(const void* src, const void* dst, int n_buckets, int n_heads, int bidirectional, int max_distance,
+                   int R, const char* what) {
+    const std::string w(what);
+    require(src && dst, w + ": NULL device pointer");
+    require(n_heads > 0 && n_heads <= 65535, w + ": n_heads must be 1 .. 65535");
+    require(n_buckets >= 4 && n_buckets <= (bidirectional ? 2 : 1) * kMaxHalf && (!bidirectional || n_buckets % 2 == 0),
+            w + ": n_buckets must be 4 .. 512 (bidirectional: even, 4 .. 1024)");
+    require(max_distance > (bidirectional ? n_buckets / 2 : n_buckets) / 2,
+            w + ": max_distance must exceed the buckets of one distance each");
+    require(R >= 1 && R <= kMaxRadius, w + ": bias_radius must be 1 .. 4096");
+}
+
+template <class T, int D, bool CAP, bool SPLIT>
+void launch_fwd(const vdk_attn_plan* p, FwdArgs a, hipStream_t s) {
+    constexpr int NW = 4;
+    const size_t lds = 4 * kKeys * D * 2 + (a.radius ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0);
+    auto kern = relpos_fwd_kernel<T, D, NW, CAP, SPLIT>;
+    if (lds > 65536)
+        VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    a.tiles = p->d_q128;
+    a.n_tiles = p->n_q128;
+    hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(64 * NW), lds, s, a);
+    VDK_HIP(hipGetLastError());
+}
+
+template <class T, int D>
+void launch_fwd_t(const vdk_attn_plan* p, const FwdArgs& a, bool cap, hipStream_t s) {
+    if (a.o32) cap ? launch_fwd<T, D, true, true>(p, a, s) : launch_fwd<T, D, false, true>(p, a, s);
+    else cap ? launch_fwd<T, D, true, false>(p, a, s) : launch_fwd<T, D, false, false>(p, a, s);
+}
+
+}  // namespace
+
+void check_rows(const void* p, long long tok, long long head, int dim, const char* name) {
+    const std::string w(name);
+    require(p, "relpos_attention: " + w + " is NULL");
+    require((uintptr_t)p % 16 == 0, "relpos_attention: " + w + " must be 16-byte aligned");
+    require(tok % 8 == 0 && head % 8 == 0 && tok >= dim && tok <= (1 << 22) && head >= 0 && head <= (1ll << 40),
+            "relpos_attention: strides of " + w + " must be multiples of 8, between tokens head_dim .. 2^22");
+}
+
+void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a) {
+    require(p && a, "relpos_attention: NULL plan or description");
+    require(a->dtype == VDK_F16 || a->dtype == VDK_BF16, "relpos_attention: dtype must be VDK_F16 or VDK_BF16");
+    require(std::isfinite(a->scale) && a->scale > 0.0f, "relpos_attention: scale must be positive and finite");
+    require(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
+            "relpos_attention: cap must be 0 or 1e-3 .. 1e6");
+    require(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= kMaxRadius),
+            "relpos_attention: bias_radius must be 1 .. 4096");
+    require((uintptr_t)a->dist_bias % 4 == 0 && (uintptr_t)a->lse % 4 == 0 && (uintptr_t)a->o_f32 % 16 == 0,
+            "relpos_attention: misaligned pointer");
+    if (p->total_q == 0) return;
+    check_rows(a->q, a->q_tok, a->q_head, p->dim, "q");
+    check_rows(a->o, a->o_tok, a->o_head, p->dim, "o");
+    if (p->total_kv > 0) {
+        check_rows(a->k, a->k_tok, a->k_head, p->dim, "k");
+        check_rows(a->v, a->v_tok, a->v_head, p->dim, "v");
+    }
+    require(p->device, "relpos_attention: the plan was made without a GPU");
+}
+
+}  // namespace vdk
+
+using namespace vdk;
+
+extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, const long long* kv_offsets, int n_heads,
+                                    int n_kv_heads, int head_dim, int causal, const long long* prefix,
+                                    vdk_attn_plan** plan) {
+    return guarded([&] {
+        require(plan, "attn_plan: NULL result pointer");
+        *plan = nullptr;
+        require(n_clips >= 0 && q_offsets && kv_offsets, "attn_plan: NULL offsets or a negative number of clips");
+        require(head_dim == 64 || head_dim == 128, "attn_plan: head_dim must be 64 or 128");
+        require(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 1024,
+                "attn_plan: n_heads must be a multiple of n_kv_heads, at most 1024");
+        require(causal || !prefix, "attn_plan: a prefix needs causal");
+        require(q_offsets[0] == 0 && kv_offsets[0] == 0, "attn_plan: offsets must start at 0");
+        vdk_attn_plan p{};
+        p.n_clips = n_clips;
+        p.n_heads = n_heads;
+        p.n_kv = n_kv_heads;
+        p.dim = head_dim;
+        p.causal = causal != 0;
+        std::vector<std::pair<long long, int2>> q128, k128;   // (work, tile)
+        int b32 = 0;
+        for (int c = 0; c < n_clips; ++c) {
+            const long long nq = q_offsets[c + 1] - q_offsets[c], nk = kv_offsets[c + 1] - kv_offsets[c];
+            require(nq >= 0 && nk >= 0 && q_offsets[c] >= 0 && kv_offsets[c] >= 0, "attn_plan: offsets must not fall");
+            require(nq <= (1 << 30) && nk <= (1 << 30), "attn_plan: a clip may hold 2^30 frames at most");
+            const long long pre = prefix ? prefix[c] : 0;
+            require(pre >= 0 && pre <= nk, "attn_plan: a prefix must be 0 .. the clip's keys");
+            p.clips.push_back({q_offsets[c], kv_offsets[c], (int)nq, (int)nk, (int)pre, b32});
+            const long long past = nk - nq;
+            auto seen = [&](long long q) { return p.causal ? std::max(0ll, std::min(nk, std::max(pre, past + q + 1))) : nk; };
+            for (long long q = 0; q < nq; q += 128)
+                q128.push_back({seen(std::min(q + 128, nq) - 1), int2{c, (int)q}});
+            b32 += cdiv(nq, 32);
+            require((long long)b32 * n_heads < (1 << 30) && k128.size() * n_heads < (1u << 30),
+                    "attn_plan: too many tiles for one launch");
+            for (long long k = 0; k < nk; k += 128) {
+                const long long first = p.causal && k >= pre ? std::max(0ll, k - past) : 0;   // the first query that sees it
+                k128.push_back({std::max(0ll, nq - first), int2{c, (int)k}});
+            }
+        }
+        p.total_q = n_clips ? q_offsets[n_clips] : 0;
+        p.total_kv = n_clips ? kv_offsets[n_clips] : 0;
+        require(p.total_q <= (1ll << 36) && p.total_kv <= (1ll << 36), "attn_plan: too many frames");
+        std::vector<int2> lists;
+        for (auto* l : {&q128, &k128}) {
+            std::stable_sort(l->begin(), l->end(), [](const auto& x, const auto& y) { return x.first > y.first; });
+            for (const auto& t : *l) lists.push_back(t.second);
+        }
+        p.n_q128 = (int)q128.size();
+        p.n_k128 = (int)k128.size();
+        p.n_b32 = b32;
+        const size_t nc = p.clips.size() * sizeof(AttnClip), nl = lists.size() * sizeof(int2);
+        if (vdk_device_count() > 0 && nc + nl > 0) {
+            VDK_HIP(hipMalloc(&p.device, nc + nl));
+            p.d_clips = static_cast<AttnClip*>(p.device);
+            p.d_q128 = reinterpret_cast<int2*>(static_cast<char*>(p.device) + nc);
+            p.d_k128 = p.d_q128 + p.n_q128;
+            try {
+                VDK_HIP(hipMemcpy(p.d_clips, p.clips.data(), nc, hipMemcpyHostToDevice));
+                VDK_HIP(hipMemcpy(p.d_q128, lists.data(), nl, hipMemcpyHostToDevice));
+                *plan = new vdk_attn_plan(p);
+            } catch (...) {
+                (void)hipFree(p.device);
+                throw;
+            }
+            return;
+        }
+        *plan = new vdk_attn_plan(p);
+    });
+}
+
+extern "C" void vdk_attn_plan_destroy(vdk_attn_plan* p) {
+    if (!p) return;
+    if (p->device) (void)hipFree(p->device);
+    delete p;
+}
+
+extern "C" int vdk_relpos_attention(const vdk_attn_plan* p, const vdk_relpos_attn* a, void* stream) {
+    return guarded([&] {
+        check_relpos(p, a);
+        if (p->total_q == 0) return;
+        FwdArgs f{a->q, a->k, a->v, a->q_tok, a->q_head, a->k_tok, a->k_head, a->v_tok, a->v_head, a->dist_bias,
+                  a->dist_bias ? a->bias_radius : 0, score_map(a->scale, a->cap), a->o, a->o_tok, a->o_head, a->o_f32,
+                  a->lse, p->d_clips, nullptr, 0, p->n_heads, p->n_heads / p->n_kv, p->causal, p->total_q};
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        if (a->dtype == VDK_F16)
+            p->dim == 64 ? launch_fwd_t<half_t, 64>(p, f, a->cap > 0, s) : launch_fwd_t<half_t, 128>(p, f, a->cap > 0, s);
+        else
+            p->dim == 64 ? launch_fwd_t<bf16_t, 64>(p, f, a->cap > 0, s) : launch_fwd_t<bf16_t, 128>(p, f, a->cap > 0, s);
+    });
+}
+
+extern "C" int vdk_rel_bias_expand(const float* d_table, int n_buckets, int n_heads, int bidirectional,
+                                   int max_distance, int bias_radius, float* d_dist_bias, void* stream) {
+    return guarded([&] {
+        check_buckets(d_table, d_dist_bias, n_buckets, n_heads, bidirectional, max_distance, bias_radius,
+                      "rel_bias_expand");
+        hipLaunchKernelGGL(rel_bias_expand_kernel, dim3(cdiv(2 * bias_radius + 1, 256), n_heads), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), d_table,
+                           buckets_of(n_buckets, bidirectional != 0, max_distance), n_heads, bias_radius, d_dist_bias);
+        VDK_HIP(hipGetLastError());
+    });
+}
+
+extern "C" int vdk_rel_bias_reduce(const float* d_dist_grad, int n_buckets, int n_heads, int bidirectional,
+                                   int max_distance, int bias_radius, float* d_table_grad, void* stream) {
+    return guarded([&] {
+        check_buckets(d_dist_grad, d_table_grad, n_buckets, n_heads, bidirectional, max_distance, bias_radius,
+                      "rel_bias_reduce");
+        hipLaunchKernelGGL(rel_bias_reduce_kernel, dim3(n_buckets, n_heads), dim3(64), 0,
+                           static_cast<hipStream_t>(stream), d_dist_grad,
+                           buckets_of(n_buckets, bidirectional != 0, max_distance), n_heads, bias_radius,
+                           d_table_grad);
+        VDK_HIP(hipGetLastError());
+    });
+}

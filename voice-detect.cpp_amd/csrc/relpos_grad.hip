@@ -1,0 +1,587 @@
+// relpos_grad.hip - gradients of the attention with a learned position bias.
+//
+// With P = exp(s - lse), delta_i = sum_d o_i dO_i (o unrounded), dP = dO V^T:
+//   dV = P^T dO, dS = P (dP - delta), d bias by distance = diagonal sums of dS,
+//   dx = dS (1 - tanh^2) with a cap, dQ = scale dx K, dK = scale dx^T Q.
+// Two kernels, each recomputing P from lse, so that no sum needs atomics: one
+// owns 128 queries (delta, dQ, the bias), one 128 keys (dK, dV; the heads that
+// share them in turn).  Seven products where one kernel with atomics has five.
+//
+// P is carried times 2^8 and, in f16, dx times a power of two that brings the
+// row's (block's) largest |dO| to 2^-4 .. 2^-3: both are rounded to 16 bits as
+// MFMA operands, and the powers keep them clear of f16's subnormal numbers.
+#include "attn.hpp"
+
+namespace vdk {
+namespace {
+
+struct GradArgs {
+    const void *q, *k, *v, *d_o;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
+    const float *o32, *lse, *bias;
+    int radius;
+    ScoreMap map;
+    float scale;
+    void *dq, *dk, *dv;
+    long long dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
+    float *delta, *most, *part, *d_dist;   // [heads][total_q], [heads][blocks], [heads][blocks][2 R + 1], the result
+    int2* span;                            // [blocks]: the distances a block of 32 queries has written
+    const AttnClip* clips;
+    const int2* tiles;
+    int n_tiles, n_heads, n_kv, group, causal, n_b32;
+    long long total_q;
+};
+
+constexpr float kPShift = 8.0f;   // P is carried times 2^8
+
+// 1 - tanh^2 from the w of the score map.
+__device__ __forceinline__ float cap_slope(float w, int wide) { return wide ? 1.0f - w * w : -4.0f * w * (1.0f + w); }
+
+// The power of two that takes `most` to 2^-12 .. 2^-11 (with P's 2^8: 2^-4 .. 2^-3).
+__device__ __forceinline__ float scale_of(float most) {
+    const int e = min(max(__builtin_amdgcn_frexp_expf(most), -100), 100);
+    return __builtin_amdgcn_ldexpf(1.0f, -11 - e);
+}
+
+template <class T>
+constexpr bool kScaled = std::is_same_v<T, half_t>;
+
+// lane i of each 16 gets lane i + N (0 past the end); N may be negative.
+template <int N>
+__device__ __forceinline__ float row_shift(float x) {
+    if constexpr (N == 0) return x;
+    constexpr int ctrl = N > 0 ? 0x100 + N : 0x110 - N;
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true));
+}
+
+// Diagonal sums of one S^T block (register r: key 8 (r / 4) + 4 hl + r % 4,
+// lane: query lr) into acc[]: acc[j] of lane (hl, lr / 16, n = lr % 16) holds
+// the distance 16 j - n + 4 hl - 16 (lr / 16).  A shift inside 16 lanes lines a
+// register's distances up; the lanes that fall out belong to the next j.
+template <int KT, int R0 = 0>
+__device__ __forceinline__ void add_diagonals(const float16v& ds, float (&acc)[5]) {
+    if constexpr (R0 < 16) {
+        constexpr int s = 32 * KT + 8 * (R0 >> 2) + (R0 & 3), sh = s & 15, j = s >> 4;
+        acc[j] += row_shift<sh>(ds[R0]);
+        if constexpr (sh != 0) acc[j + 1] += row_shift<sh - 16>(ds[R0]);
+        add_diagonals<KT, R0 + 1>(ds, acc);
+    }
+}
+
+// dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32.
+template <class T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int NW = 4, kTile = kKeys * D * 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
+    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int h = id / a.n_tiles;
+    const int2 tile = a.tiles[id - h * a.n_tiles];
+    const AttnClip c = a.clips[tile.x];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
+              hl = lane >> 5;
+    const int past = c.nk - c.nq, qw = tile.y + 32 * wave, qi = qw + lr;
+    const int qr = qi < c.nq ? qi : c.nq - 1;
+    auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
+    const int kend = max(last(min(tile.y + 32 * NW, c.nq) - 1), 0);
+    const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
+    const int kfull = qw < c.nq ? last(qw) : 0;
+    const int lim = last(qr);
+
+    const uint32_t kb_row = (uint32_t)a.k_tok * 2, vb_row = (uint32_t)a.v_tok * 2;
+    const T* kp = static_cast<const T*>(a.k) + c.k0 * a.k_tok + (long long)(h / a.group) * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + c.k0 * a.v_tok + (long long)(h / a.group) * a.v_head;
+    TileDma<D, kKeys, NW> dk, dv;
+    dk.init(kb_row, wave, lane);
+    dv.init(vb_row, wave, lane);
+    auto fetch = [&](int kb, int buf) {
+        dk.load(smem + buf * 2 * kTile, kp + (long long)kb * a.k_tok, kb_row, c.nk - kb, wave);
+        dv.load(smem + buf * 2 * kTile + kTile, vp + (long long)kb * a.v_tok, vb_row, c.nk - kb, wave);
+    };
+    if (kend > 0) fetch(0, 0);
+
+    // the row's q, dO, delta and largest |dO|
+    const T* qp = static_cast<const T*>(a.q) + (c.q0 + qr) * a.q_tok + (long long)h * a.q_head;
+    const T* dp = static_cast<const T*>(a.d_o) + (c.q0 + qr) * a.do_tok + (long long)h * a.do_head;
+    const float* op = a.o32 + ((c.q0 + qr) * a.n_heads + h) * D;
+    V8 qf[D / 16], df[D / 16];
+    float delta = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk] = *reinterpret_cast<const V8*>(qp + 16 * kk + 8 * hl);
+        df[kk] = *reinterpret_cast<const V8*>(dp + 16 * kk + 8 * hl);
+        const float4v o0 = *reinterpret_cast<const float4v*>(op + 16 * kk + 8 * hl),
+                      o1 = *reinterpret_cast<const float4v*>(op + 16 * kk + 8 * hl + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float d = (float)df[kk][e];
+            delta = __builtin_fmaf(d, e < 4 ? o0[e & 3] : o1[e & 3], delta);
+            most = fmaxf(most, fabsf(d));
+        }
+    }
+    delta += other_half(delta);
+    most = fmaxf(most, other_half(most));
+    const float lse = a.lse[h * a.total_q + c.q0 + qr];
+    const float L2 = qi < c.nq && !(lse < -1e30f) ? lse * kLog2e - kPShift : FLT_MAX;
+    const float sc = kScaled<T> ? scale_of(most) : 0x1p-8f, nd = -delta * sc;
+    if (qi < c.nq && hl == 0) a.delta[h * a.total_q + c.q0 + qi] = delta;
+    if (qw < c.nq) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        if (lane == 0) a.most[h * a.n_b32 + c.b32 + (qw >> 5)] = most;
+    }
+    const int R = BIAS ? a.radius : 0;
+    float far_l = a.map.ab, far_r = a.map.ab;
+    if constexpr (BIAS) {
+        const float* b = a.bias + (long long)h * (2 * R + 1);
+        for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]) + a.map.ab;
+        far_l += bias2_of(b[0]);
+        far_r += bias2_of(b[2 * R]);
+    }
+    // the bias's gradient: a ring of 128 distances for each 16 lanes, see flush
+    float* ring = tab + 2 * R + 1 + 2 * kTabPad + (3 - (2 * R + 2 * kTabPad) % 4) + wave * 512;
+    float acc[5] = {0, 0, 0, 0, 0}, left = 0.0f, right = 0.0f;
+    int lo = 1 << 30, hi = -(1 << 30);
+    float* part = nullptr;
+    if constexpr (BIAS) {
+        part = a.part + ((long long)h * a.n_b32 + c.b32 + (qw >> 5)) * (2 * R + 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ring[64 * i + lane] = 0.0f;
+    }
+    // acc[0..3] hold all that their 16 lanes add to the 64 distances from d0 - 15 (+ 4 hl - 16 (lr / 16)): stored, and
+    // the 64 distances from d0 - 31, which no later tile reaches, summed over the four sixteens and written out
+    auto flush = [&](int d0) {
+        const int rho = lane >> 4, off = 4 * hl - 16 * (rho & 1) - (lane & 15);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ring[128 * rho + ((d0 + off + 16 * j) & 127)] = acc[j];
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        const int d = d0 - 31 + lane;
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v += ring[128 * i + (d & 127)];
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (d <= -R) left += v;
+        else if (d >= R) right += v;
+        else part[d + R] = v;
+        acc[0] = acc[4];
+        acc[1] = acc[2] = acc[3] = acc[4] = 0.0f;
+    };
+
+    float16v dq[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dq[dt] = splat16(0.0f);
+    const float am = a.map.am;
+    const float unscale = kScaled<T> ? 1.0f / sc * 0x1p-8f : 1.0f;   // of dS, per row (a power of two)
+    for (int kb = 0, buf = 0; kb < kend; kb += kKeys, buf ^= 1) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
+        if (kb >= kend_w) continue;
+        const uint8_t* sk = smem + buf * 2 * kTile;
+        const uint8_t* sv = sk + kTile;
+        const int d0 = kb - (qw + past);
+        const bool near = BIAS && d0 + 63 > -R && d0 - 31 < R;
+        const float add = (d0 < 0 ? far_l : far_r) - L2;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            float16v s = splat16(0.0f), p = splat16(0.0f);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(tile_rows<T, D>(sk, 32 * kt, kk, lane), qf[kk], s);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(tile_rows<T, D>(sv, 32 * kt, kk, lane), df[kk], p);
+            score_w<CAP>(s, a.map);
+            float16v ds;
+            if (near) {
+                const float* t = tab + (d0 + 32 * kt - lr + 4 * hl + R + kTabPad);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, t[8 * (r >> 2) + (r & 3)]) - L2);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, add));
+            }
+            if (kb + kKeys > kfull) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (kb + 32 * kt + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) ds[r] = 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] *= __builtin_fmaf(p[r], sc, nd);
+            if constexpr (BIAS) {
+                float16v db = ds;
+                if constexpr (kScaled<T>) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) db[r] *= unscale;
+                }
+                if (near) {
+                    kt == 0 ? add_diagonals<0>(db, acc) : add_diagonals<1>(db, acc);
+                } else {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum += db[r];
+                    if (d0 < 0) left += sum;
+                    else right += sum;
+                }
+            }
+            if constexpr (CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] *= cap_slope(s[r], a.map.wide);
+            }
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+                const V8 pb = pack8<T>(ds, cc);
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt)
+                    dq[dt] = mfma32(tr_pair<T, D>(sk, 32 * kt + 16 * cc, dt, lane), pb, dq[dt]);
+            }
+        }
+        if constexpr (BIAS) {
+            if (near) {
+                lo = min(lo, d0 - 31);
+                hi = d0 + 96;
+                flush(d0);
+                if (kb + kKeys >= kend_w || d0 + 64 - 31 >= R) flush(d0 + 64);   // the last one: what is left
+            }
+        }
+    }
+    if constexpr (BIAS) {
+        if (qw < c.nq) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                left += __shfl_xor(left, off, 64);
+                right += __shfl_xor(right, off, 64);
+            }
+            if (lane == 0) {
+                part[0] = left;
+                part[2 * R] = right;
+                if (h == 0) a.span[c.b32 + (qw >> 5)] = int2{lo, hi};
+            }
+        }
+    }
+    if (qi >= c.nq) return;
+    const float f = a.scale * 0x1p-8f / sc;   // undo 2^8 and sc (both powers of two)
+    T* out = static_cast<T*>(a.dq) + (c.q0 + qi) * a.dq_tok + (long long)h * a.dq_head;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const auto u0 = pack2<T>(dq[dt][4 * g] * f, dq[dt][4 * g + 1] * f),
+                       u1 = pack2<T>(dq[dt][4 * g + 2] * f, dq[dt][4 * g + 3] * f);
+            *reinterpret_cast<uint2*>(out + 32 * dt + 8 * g + 4 * hl) =
+                uint2{__builtin_bit_cast(uint32_t, u0), __builtin_bit_cast(uint32_t, u1)};
+        }
+}
+
+// dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 queries a step
+// through LDS, the heads that share the keys one after the other.
+template <class T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void relpos_dkv_kernel(GradArgs a) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int NW = 4, kTile = kKeys * D * 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: ab - L2 and -delta sc of a step's queries
+    float* tab = rows + 256;
+    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int kvh = id / a.n_tiles;
+    const int2 tile = a.tiles[id - kvh * a.n_tiles];
+    const AttnClip c = a.clips[tile.x];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
+              hl = lane >> 5;
+    const int past = c.nk - c.nq, kw = tile.y + 32 * wave, ki = kw + lr;
+    const int kr = ki < c.nk ? ki : c.nk - 1;
+    // the first query that sees a key of the tile, down to a whole step
+    const int q_first = a.causal && tile.y >= c.prefix ? max(tile.y - past, 0) & ~63 : 0;
+    const int per_head = q_first < c.nq ? (c.nq - q_first + 63) >> 6 : 0, steps = per_head * a.group;
+
+    const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + (c.k0 + kr) * a.v_tok + (long long)kvh * a.v_head;
+    V8 kf[D / 16], vf[D / 16];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        kf[kk] = *reinterpret_cast<const V8*>(kp + 16 * kk + 8 * hl);
+        vf[kk] = *reinterpret_cast<const V8*>(vp + 16 * kk + 8 * hl);
+    }
+    const uint32_t qb_row = (uint32_t)a.q_tok * 2, db_row = (uint32_t)a.do_tok * 2;
+    TileDma<D, kKeys, NW> dmq, dmo;
+    dmq.init(qb_row, wave, lane);
+    dmo.init(db_row, wave, lane);
+    float row_v = 0.0f;   // this thread's entry of the next step's rows[]
+    auto step_scale = [&](int h, int q) {   // from the step's largest |dO|
+        if constexpr (!kScaled<T>) return 0x1p-8f;
+        const float* p = a.most + h * a.n_b32 + c.b32 + (q >> 5);
+        return scale_of(q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
+    };
+    auto fetch = [&](int it, int buf) {
+        const int h = kvh * a.group + it / per_head, q = q_first + (it % per_head) * 64;
+        const T* qs = static_cast<const T*>(a.q) + (c.q0 + q) * a.q_tok + (long long)h * a.q_head;
+        const T* ds = static_cast<const T*>(a.d_o) + (c.q0 + q) * a.do_tok + (long long)h * a.do_head;
+        dmq.load(smem + buf * 2 * kTile, qs, qb_row, c.nq - q, wave);
+        dmo.load(smem + buf * 2 * kTile + kTile, ds, db_row, c.nq - q, wave);
+        if (threadIdx.x < 128) {
+            const int qi = q + (threadIdx.x & 63);
+            const long long at = h * a.total_q + c.q0 + min(qi, c.nq - 1);
+            if (threadIdx.x < 64) {
+                const float lse = a.lse[at];
+                row_v = qi < c.nq && !(lse < -1e30f) ? a.map.ab + kPShift - lse * kLog2e : -FLT_MAX;
+            } else {
+                row_v = qi < c.nq ? -a.delta[at] * step_scale(h, q) : 0.0f;
+            }
+        }
+    };
+    if (steps > 0) fetch(0, 0);
+    const int R = BIAS ? a.radius : 0;
+
+    float16v dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = splat16(0.0f);
+    const float am = a.map.am;
+    float sc = 0x1p-8f, far_l = 0.0f, far_r = 0.0f;
+    if constexpr (kScaled<T>) {
+        if (steps > 0) sc = step_scale(kvh * a.group, q_first);
+    }
+    for (int it = 0, buf = 0; it < steps; ++it, buf ^= 1) {
+        const int hg = it / per_head, h = kvh * a.group + hg, q = q_first + (it % per_head) * 64;
+        if constexpr (BIAS) {
+            if (it % per_head == 0) {   // another head's bias
+                lds_barrier();
+                const float* b = a.bias + (long long)h * (2 * R + 1);
+                for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+                    tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
+                far_l = bias2_of(b[0]);
+                far_r = bias2_of(b[2 * R]);
+            }
+        }
+        if (threadIdx.x < 128) rows[buf * 128 + threadIdx.x] = row_v;
+        wait_vmcnt<0>();
+        lds_barrier();
+        const float* nl = rows + buf * 128;
+        const float* nd = nl + 64;
+        if (it + 1 < steps) fetch(it + 1, buf ^ 1);
+        if constexpr (kScaled<T>) {   // dK is carried in the scale of the step: moved with it, exactly
+            const float s_new = step_scale(h, q);
+            if (s_new != sc) {
+                const float f = s_new / sc;
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dk[dt][r] *= f;
+                sc = s_new;
+            }
+        }
+        const uint8_t* sq = smem + buf * 2 * kTile;
+        const uint8_t* so = sq + kTile;
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt) {
+            const int qs = q + 32 * qt;
+            if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
+            float16v s = splat16(0.0f), p = splat16(0.0f);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(tile_rows<T, D>(sq, 32 * qt, kk, lane), kf[kk], s);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(tile_rows<T, D>(so, 32 * qt, kk, lane), vf[kk], p);
+            score_w<CAP>(s, a.map);
+            // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki
+            const int d0 = kw - (qs + past);   // distances d0 - 31 .. d0 + 31
+            const bool near = BIAS && d0 + 31 > -R && d0 - 31 < R;
+            float16v pr, ds;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4v l4 = *reinterpret_cast<const float4v*>(nl + 32 * qt + 8 * g + 4 * hl);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[4 * g + e] = l4[e];
+            }
+            if (near) {
+                const float* t = tab + (d0 + lr - 4 * hl + R + kTabPad);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, t[-(8 * (r >> 2) + (r & 3))]) + pr[r]);
+            } else if (BIAS) {
+                const float far = d0 < 0 ? far_l : far_r;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, far) + pr[r]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, pr[r]));
+            }
+            if (a.causal && kw + 31 >= max(c.prefix, past + qs + 1)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (ki >= max(c.prefix, past + qs + 8 * (r >> 2) + 4 * hl + (r & 3) + 1)) pr[r] = 0.0f;
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4v d4 = *reinterpret_cast<const float4v*>(nd + 32 * qt + 8 * g + 4 * hl);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    ds[4 * g + e] = pr[4 * g + e] * __builtin_fmaf(p[4 * g + e], sc, d4[e]);
+            }
+            if constexpr (CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] *= cap_slope(s[r], a.map.wide);
+            }
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+                const V8 pb = pack8<T>(pr, cc), db = pack8<T>(ds, cc);
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt) {
+                    dv[dt] = mfma32(tr_pair<T, D>(so, 32 * qt + 16 * cc, dt, lane), pb, dv[dt]);
+                    dk[dt] = mfma32(tr_pair<T, D>(sq, 32 * qt + 16 * cc, dt, lane), db, dk[dt]);
+                }
+            }
+        }
+    }
+    if (ki >= c.nk) return;
+    const float f = a.scale * 0x1p-8f / sc;
+    T* ok = static_cast<T*>(a.dk) + (c.k0 + ki) * a.dk_tok + (long long)kvh * a.dk_head;
+    T* ov = static_cast<T*>(a.dv) + (c.k0 + ki) * a.dv_tok + (long long)kvh * a.dv_head;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * dt + 8 * g + 4 * hl;
+            auto put = [&](T* out, const float16v& x, float m) {
+                const auto u0 = pack2<T>(x[4 * g] * m, x[4 * g + 1] * m), u1 = pack2<T>(x[4 * g + 2] * m, x[4 * g + 3] * m);
+                *reinterpret_cast<uint2*>(out + d) =
+                    uint2{__builtin_bit_cast(uint32_t, u0), __builtin_bit_cast(uint32_t, u1)};
+            };
+            put(ok, dk[dt], f);
+            put(ov, dv[dt], 0x1p-8f);
+        }
+}
+
+// The blocks' partial sums of 64 distances, 16 rows of blocks at a time, in a fixed order.
+__global__ __launch_bounds__(1024) void relpos_dbias_kernel(GradArgs a) {
+    __shared__ double red[16][64];
+    const int R = a.radius, h = blockIdx.y, i = blockIdx.x * 64 + (threadIdx.x & 63), row = threadIdx.x >> 6;
+    double sum = 0.0;
+    if (i <= 2 * R) {
+        const bool edge = i == 0 || i == 2 * R;
+        for (int b = row; b < a.n_b32; b += 16) {
+            const int2 s = a.span[b];
+            if (edge || (i - R >= s.x && i - R <= s.y)) sum += a.part[((long long)h * a.n_b32 + b) * (2 * R + 1) + i];
+        }
+    }
+    red[row][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (row == 0 && i <= 2 * R) {
+        sum = 0.0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += red[r][threadIdx.x];
+        a.d_dist[(long long)h * (2 * R + 1) + i] = (float)sum;
+    }
+}
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+template <class T, int D, bool CAP, bool BIAS>
+void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
+    const int tab = BIAS ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0;
+    const int tiles = 4 * kKeys * D * 2;
+    if (p->n_q128) {
+        auto kern = relpos_dq_kernel<T, D, CAP, BIAS>;
+        const int lds = tiles + (BIAS ? tab + 16 + 4 * 512 * 4 : 0);
+        if (lds > 65536)
+            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        a.tiles = p->d_q128;
+        a.n_tiles = p->n_q128;
+        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(256), lds, s, a);
+        VDK_HIP(hipGetLastError());
+    }
+    if (p->n_k128) {
+        auto kern = relpos_dkv_kernel<T, D, CAP, BIAS>;
+        const int lds = tiles + 1024 + tab;
+        if (lds > 65536)
+            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        a.tiles = p->d_k128;
+        a.n_tiles = p->n_k128;
+        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_kv), dim3(256), lds, s, a);
+        VDK_HIP(hipGetLastError());
+    }
+    if (a.d_dist) {
+        hipLaunchKernelGGL(relpos_dbias_kernel, dim3(cdiv(2 * a.radius + 1, 64), a.n_heads), dim3(1024), 0, s, a);
+        VDK_HIP(hipGetLastError());
+    }
+}
+
+template <class T, int D>
+void launch_grad_t(const vdk_attn_plan* p, const GradArgs& a, bool cap, hipStream_t s) {
+    if (a.radius) cap ? launch_grad<T, D, true, true>(p, a, s) : launch_grad<T, D, false, true>(p, a, s);
+    else cap ? launch_grad<T, D, true, false>(p, a, s) : launch_grad<T, D, false, false>(p, a, s);
+}
+
+}  // namespace
+}  // namespace vdk
+
+using namespace vdk;
+
+extern "C" size_t vdk_relpos_attention_backward_workspace_size(const vdk_attn_plan* p, int bias_radius) {
+    size_t n = 0;
+    if (guarded([&] {
+            require(p, "relpos_attention_backward: NULL plan");
+            require(bias_radius >= 0 && bias_radius <= 4096, "relpos_attention_backward: bias_radius must be 0 .. 4096");
+            n = up16((size_t)p->n_heads * p->total_q * 4) + up16((size_t)p->n_heads * p->n_b32 * 4) +
+                up16((size_t)p->n_b32 * sizeof(int2)) +
+                (bias_radius ? (size_t)p->n_heads * p->n_b32 * (2 * bias_radius + 1) * 4 : 0);
+        }) != 0)
+        return 0;
+    return up16(n);
+}
+
+extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_relpos_attn* a,
+                                             const vdk_relpos_attn_grad* g, void* stream) {
+    return guarded([&] {
+        check_relpos(p, a);
+        require(g, "relpos_attention_backward: NULL description");
+        require(!g->d_dist_bias || a->dist_bias, "relpos_attention_backward: d_dist_bias without a bias");
+        require((uintptr_t)g->d_dist_bias % 4 == 0, "relpos_attention_backward: misaligned pointer");
+        const int R = a->dist_bias ? a->bias_radius : 0;
+        if (p->total_q > 0) {
+            require(a->o_f32 && a->lse, "relpos_attention_backward: o_f32 and lse of the forward call are missing");
+            check_rows(g->d_o, g->do_tok, g->do_head, p->dim, "d_o");
+            check_rows(g->dq, g->dq_tok, g->dq_head, p->dim, "dq");
+        }
+        if (p->total_kv > 0) {
+            check_rows(g->dk, g->dk_tok, g->dk_head, p->dim, "dk");
+            check_rows(g->dv, g->dv_tok, g->dv_head, p->dim, "dv");
+            require(p->device, "relpos_attention: the plan was made without a GPU");
+        }
+        const size_t need = vdk_relpos_attention_backward_workspace_size(p, R);
+        require(need == 0 || (g->work && g->work_bytes >= need && (uintptr_t)g->work % 16 == 0),
+                "relpos_attention_backward: workspace missing, misaligned or too small");
+        GradArgs f{};
+        f.q = a->q; f.k = a->k; f.v = a->v; f.d_o = g->d_o;
+        f.q_tok = a->q_tok; f.q_head = a->q_head; f.k_tok = a->k_tok; f.k_head = a->k_head;
+        f.v_tok = a->v_tok; f.v_head = a->v_head; f.do_tok = g->do_tok; f.do_head = g->do_head;
+        f.o32 = a->o_f32; f.lse = a->lse; f.bias = a->dist_bias; f.radius = R;
+        f.map = score_map(a->scale, a->cap);
+        f.scale = a->scale;
+        f.dq = g->dq; f.dk = g->dk; f.dv = g->dv;
+        f.dq_tok = g->dq_tok; f.dq_head = g->dq_head; f.dk_tok = g->dk_tok; f.dk_head = g->dk_head;
+        f.dv_tok = g->dv_tok; f.dv_head = g->dv_head;
+        uint8_t* w = static_cast<uint8_t*>(g->work);
+        f.delta = reinterpret_cast<float*>(w);
+        w += up16((size_t)p->n_heads * p->total_q * 4);
+        f.most = reinterpret_cast<float*>(w);
+        w += up16((size_t)p->n_heads * p->n_b32 * 4);
+        f.span = reinterpret_cast<int2*>(w);
+        w += up16((size_t)p->n_b32 * sizeof(int2));
+        f.part = reinterpret_cast<float*>(w);
+        f.d_dist = g->d_dist_bias;
+        f.clips = p->d_clips;
+        f.n_heads = p->n_heads;
+        f.n_kv = p->n_kv;
+        f.group = p->n_heads / p->n_kv;
+        f.causal = p->causal;
+        f.n_b32 = p->n_b32;
+        f.total_q = p->total_q;
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        if (a->dtype == VDK_F16) p->dim == 64 ? launch_grad_t<half_t, 64>(p, f, a->cap > 0, s)
+                                              : launch_grad_t<half_t, 128>(p, f, a->cap > 0, s);
+        else p->dim == 64 ? launch_grad_t<bf16_t, 64>(p, f, a->cap > 0, s)
+                          : launch_grad_t<bf16_t, 128>(p, f, a->cap > 0, s);
+    });
+}

@@ -28,6 +28,49 @@ class FbankCfg(C.Structure):
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_GELU, ACT_TANH = 0, 1, 2, 3, 4, 5
 
 
+F16, BF16 = 0, 1
+KV_16, KV_E4M3 = 0, 1
+STATUS_BAD_SLOT, STATUS_BAD_PAGE, STATUS_BAD_LENGTH = 1, 2, 4
+_ll = C.c_longlong
+
+
+class RelposAttn(C.Structure):
+    """vdk_relpos_attn (include/vdk.h)."""
+    _fields_ = [("dtype", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
+                ("q", _vp), ("q_tok", _ll), ("q_head", _ll),
+                ("k", _vp), ("k_tok", _ll), ("k_head", _ll),
+                ("v", _vp), ("v_tok", _ll), ("v_head", _ll),
+                ("dist_bias", _vp), ("bias_radius", C.c_int),
+                ("o", _vp), ("o_tok", _ll), ("o_head", _ll),
+                ("o_f32", _vp), ("lse", _vp)]
+
+
+class RelposAttnGrad(C.Structure):
+    """vdk_relpos_attn_grad (include/vdk.h)."""
+    _fields_ = [("d_o", _vp), ("do_tok", _ll), ("do_head", _ll),
+                ("dq", _vp), ("dq_tok", _ll), ("dq_head", _ll),
+                ("dk", _vp), ("dk_tok", _ll), ("dk_head", _ll),
+                ("dv", _vp), ("dv_tok", _ll), ("dv_head", _ll),
+                ("d_dist_bias", _vp), ("work", _vp), ("work_bytes", C.c_size_t)]
+
+
+class KvCache(C.Structure):
+    """vdk_kv_cache (include/vdk.h)."""
+    _fields_ = [("dtype", C.c_int), ("format", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class PagedAttn(C.Structure):
+    """vdk_paged_attn (include/vdk.h)."""
+    _fields_ = [("n_seqs", C.c_int), ("n_q_heads", C.c_int), ("max_pages", C.c_int), ("max_len", C.c_int),
+                ("q", _vp), ("q_seq", _ll), ("q_head", _ll),
+                ("block_table", _vp), ("seq_lens", _vp), ("scale", C.c_float), ("cap", C.c_float),
+                ("dist_bias", _vp), ("bias_radius", C.c_int),
+                ("o", _vp), ("o_seq", _ll), ("o_head", _ll), ("lse", _vp),
+                ("work", _vp), ("work_bytes", C.c_size_t), ("status", _vp)]
+
+
 class Res2Weights(C.Structure):
     """vdk_res2_weights (include/vdk.h)."""
     _fields_ = [("w", _vp * 7), ("bias", _vp * 7), ("scale", _vp * 7), ("shift", _vp * 7)]
@@ -195,6 +238,18 @@ _SIGS = {
     "vdk_conv_tuned_tile": (C.c_int, [C.POINTER(ConvDesc)]),
     "vdk_cam_context": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, _vp, C.c_int,
                                   _vp, _vp]),
+    "vdk_attn_plan_create": (C.c_int, [C.c_int, C.POINTER(_ll), C.POINTER(_ll), C.c_int, C.c_int, C.c_int, C.c_int,
+                                       C.POINTER(_ll), C.POINTER(_vp)]),
+    "vdk_attn_plan_destroy": (None, [_vp]),
+    "vdk_relpos_attention": (C.c_int, [_vp, C.POINTER(RelposAttn), _vp]),
+    "vdk_relpos_attention_backward_workspace_size": (C.c_size_t, [_vp, C.c_int]),
+    "vdk_relpos_attention_backward": (C.c_int, [_vp, C.POINTER(RelposAttn), C.POINTER(RelposAttnGrad), _vp]),
+    "vdk_rel_bias_expand": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]),
+    "vdk_rel_bias_reduce": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]),
+    "vdk_kv_cache_write": (C.c_int, [C.POINTER(KvCache), _vp, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp]),
+    "vdk_kv_cache_read": (C.c_int, [C.POINTER(KvCache), _vp, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp]),
+    "vdk_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(PagedAttn)]),
+    "vdk_paged_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(PagedAttn), _vp]),
 }
 
 
@@ -268,6 +323,34 @@ class DeviceBuffer:
 
 def check(rc):
     _ok(rc)
+
+
+class AttnPlan:
+    """Owning wrapper over a vdk_attn_plan: the layout of packed clips for vdk_relpos_attention."""
+
+    def __init__(self, q_offsets, kv_offsets, n_heads, n_kv_heads, head_dim, causal=False, prefix=None):
+        self.ptr = None
+        n = len(q_offsets) - 1
+        if n < 0 or len(kv_offsets) != n + 1 or (prefix is not None and len(prefix) != n):
+            raise ValueError("AttnPlan: q_offsets and kv_offsets need one entry more than clips, prefix one a clip")
+        if prefix is not None and not any(prefix):
+            prefix = None
+        p = _vp()
+        _ok(lib().vdk_attn_plan_create(n, (_ll * (n + 1))(*q_offsets), (_ll * (n + 1))(*kv_offsets), n_heads,
+                                       n_kv_heads, head_dim, int(causal),
+                                       None if prefix is None else (_ll * n)(*prefix), C.byref(p)))
+        self.ptr = p.value
+
+    def close(self):
+        if self.ptr:
+            lib().vdk_attn_plan_destroy(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Context:
