@@ -66,18 +66,23 @@ __device__ __forceinline__ float16v splat16(float x) {
     return v;
 }
 
-// What pack8 rounded away, rounded itself: the two together hold twice the bits.
+// The same registers less their rounded values v: what is still to be carried.
 template <class T>
-__device__ __forceinline__ typename Vec8<T>::type rest8(const float16v& s, typename Vec8<T>::type hi, int c) {
-    typename Vec8<T>::type v;
+__device__ __forceinline__ void take8(float16v& s, typename Vec8<T>::type v, int c) {
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const auto p = pack2<T>(s[8 * c + j] - (float)hi[j], s[8 * c + j + 1] - (float)hi[j + 1]);
-        v[j] = p[0];
-        v[j + 1] = p[1];
-    }
-    return v;
+    for (int j = 0; j < 8; ++j) s[8 * c + j] -= (float)v[j];
 }
+
+// The largest of three (no operand is a signalling NaN, which fmaxf would see to).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// Inside an `if` that is rarely taken and the same for the whole wave: keeps the
+// compiler from turning the branch into selects that every step would pay for.
+__device__ __forceinline__ void keep_branch() { asm volatile("; rare"); }
 
 // The other 32 lanes' value.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
@@ -141,42 +146,58 @@ __device__ __forceinline__ typename Vec8<T>::type tr_pair(const uint8_t* lds, in
 }
 
 // ---- scores ----
-// Scores are kept in units of log 2: s2 = am * w + ab + bias2, with w = q . k
-// without a cap.  With one, tanh(y) = 1 - 2 / (1 + exp(2 y)) takes w = -1 / (1 +
-// exp(2 y)): one exp2, one add, one reciprocal.  Its error is that of a 32-bit
-// rounding near 1 (6e-8 cap), so caps above 64 take w = tanh(y) from a series
-// where |y| is small instead.
+// Scores are kept in units of log 2: s2 = am * w + bias2, with w = q . k without
+// a cap, else w = tanh(y), y = scale q . k / cap.  tanh(y) / y is an even function:
+// for |y| <= 1/2 a polynomial in y^2 (Chebyshev fit, 2.7e-8 relative) keeps the
+// score's relative precision, where 1 - 2 / (1 + exp(2 y)) would lose all below
+// 6e-8 cap.  Blocks with a larger |y| take both and choose by element.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kWideCap = 64.0f;
 
 struct ScoreMap {
-    float mul, am, ab;   // mul: q . k to the exponent (or y)
-    int wide;
+    float mul, am, lim;   // q . k to y; w to s2; the |q . k| where |y| = 1/2
 };
 
 inline ScoreMap score_map(float scale, float cap) {
-    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f, 0};
-    if (cap > kWideCap) return {scale / cap, cap * kLog2e, 0.0f, 1};
-    return {2.0f * kLog2e * scale / cap, 2.0f * cap * kLog2e, cap * kLog2e, 0};
+    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f};
+    return {scale / cap, cap * kLog2e, 0.5f * cap / scale};
 }
 
-__device__ __forceinline__ float tanh_series(float y) {
-    const float y2 = y * y;
-    const float t = y * (1.0f + y2 * (-1.0f / 3 + y2 * (2.0f / 15 + y2 * (-17.0f / 315 + y2 * (62.0f / 2835)))));
+__device__ __forceinline__ float tanh_small(float y) {
+    const float z = y * y;
+    return y * __builtin_fmaf(
+                   z,
+                   __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 0.01714132f, -0.05298924f), 0.13324828f),
+                                  -0.33333072f),
+                   1.0f);
+}
+
+__device__ __forceinline__ float tanh_any(float y) {
     const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * y);
-    return fabsf(y) < 0.25f ? t : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+    return fabsf(y) < 0.5f ? tanh_small(y) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// The largest of |a|, |b| and c.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 // q . k of a block to w, in place.
-template <bool CAP>
-__device__ __forceinline__ void score_w(float16v& s, const ScoreMap& m) {
+template <bool CAP, class V>
+__device__ __forceinline__ void score_w(V& s, const ScoreMap& m) {
     if constexpr (CAP) {
-        if (m.wide) {
+        constexpr int N = sizeof(V) / 4;
+        float top = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = tanh_series(s[r] * m.mul);
+        for (int r = 0; r < N; r += 2) top = max3_abs(s[r], s[r + 1], top);
+        if (__any(top > m.lim)) {
+            keep_branch();
+#pragma unroll
+            for (int r = 0; r < N; ++r) s[r] = tanh_any(s[r] * m.mul);
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[r] * m.mul));
+            for (int r = 0; r < N; ++r) s[r] = tanh_small(s[r] * m.mul);
         }
     }
 }

@@ -292,18 +292,18 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
                     s[t] = mfma16(*reinterpret_cast<const V8*>(sk + row * kRow + 16 * ring_chunk<kRow>(row, 4 * kk + g)),
                                   qf[kk], s[t]);
             }
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][r] *= sc[16 * t + 4 * g + r];
+            }
+            score_w<CAP>(s[t], a.map);
             const int kt = kb + 16 * t + 4 * g;
             there[t] = pages[(min(kb + 16 * t, k1 - 1) >> a.page_shift) - p0] >= 0;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float w = s[t][r];
-                if constexpr (QUANT) w *= sc[16 * t + 4 * g + r];
-                if constexpr (CAP)
-                    w = a.map.wide ? tanh_series(w * a.map.mul)
-                                   : __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(w * a.map.mul));
                 const int d = min(max(kt + r - (len - 1), -a.radius), 0) + a.radius;   // (keys past the last: hidden)
                 const float b2 = bias ? bias2_of(bias[d]) : 0.0f;
-                w = __builtin_fmaf(w, a.map.am, a.map.ab + b2);
+                const float w = __builtin_fmaf(s[t][r], a.map.am, b2);
                 s[t][r] = there[t] && kt + r < k1 ? w : -INFINITY;
                 mx = fmaxf(mx, s[t][r]);
             }

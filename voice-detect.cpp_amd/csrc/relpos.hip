@@ -30,11 +30,12 @@ struct FwdArgs {
 // row's running maximum moves only when it grows by more than 8 (p <= 2^8, and
 // 16-bit p keep their relative precision), and each lane sums its own keys.
 // P^T then is the B operand of O^T += V^T P^T, V^T read by transposing LDS loads.
-// SPLIT (training, where o_f32 is wanted): P enters in two 16-bit parts, since
-// the backward pass takes delta = sum(o dO) from o, and a bias's gradient sums
-// dS over many rows, where errors of 2^-9 in P would show in a 32-bit result.
+// SPLIT (training, where o_f32 is wanted): P enters in 16-bit parts, two of f16
+// or three of bf16, 22 or 24 bits of it.  The backward pass takes delta = sum(o
+// dO) from o, and a bias's gradient sums dS over whole rows, where its terms
+// cancel and delta's error does not.
 template <class T, int D, int NW, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void relpos_fwd_kernel(FwdArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -72,13 +73,13 @@ __global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const V8*>(qp + 16 * kk + 8 * hl);
     const int R = a.radius;
-    float far_l = a.map.ab, far_r = a.map.ab;
+    float far_l = 0.0f, far_r = 0.0f;
     if (R) {
         const float* b = a.bias + (long long)h * (2 * R + 1);
         for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
-            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]) + a.map.ab;
-        far_l += bias2_of(b[0]);
-        far_r += bias2_of(b[2 * R]);
+            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
+        far_l = bias2_of(b[0]);
+        far_r = bias2_of(b[2 * R]);
     }
 
     float16v o[D / 32];
@@ -103,6 +104,7 @@ __global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
         }
         // s[kt][r]: key kb + 32 kt + 8 (r / 4) + 4 hl + r % 4 of query qi
         if (kb + kKeys > kfull) {
+            keep_branch();
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -122,6 +124,7 @@ __global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
             mul = 1.0f;
             add = 0.0f;
         } else if (add < -1e37f) {   // a far bias of the lowest value takes the products in, as the near ones do
+            keep_branch();
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -129,11 +132,15 @@ __global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
             mul = 1.0f;
             add = 0.0f;
         }
-        float mx = s[0][0];
+        float mx = max3(s[0][0], s[0][1], s[1][0]);
 #pragma unroll
-        for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        for (int r = 2; r < 16; r += 2) mx = max3(mx, s[0][r], s[0][r + 1]);
+#pragma unroll
+        for (int r = 1; r < 15; r += 2) mx = max3(mx, s[1][r], s[1][r + 1]);
+        mx = max3(mx, s[1][15], mx);
         mx = __builtin_fmaf(fmaxf(mx, other_half(mx)), mul, add);
         if (__any(mx > m + 8.0f)) {
+            keep_branch();
             const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
             l *= alpha;
@@ -153,12 +160,18 @@ __global__ __launch_bounds__(64 * NW) void relpos_fwd_kernel(FwdArgs a) {
             }
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-            const V8 pb = pack8<T>(s[cc >> 1], cc & 1);
+            constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
+            V8 pb[kParts];
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                pb[i] = pack8<T>(s[cc >> 1], cc & 1);
+                if (i + 1 < kParts) take8<T>(s[cc >> 1], pb[i], cc & 1);
+            }
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt) {
                 const V8 vt = tr_pair<T, D>(sv, 16 * cc, dt, lane);
-                o[dt] = mfma32(vt, pb, o[dt]);
-                if constexpr (SPLIT) o[dt] = mfma32(vt, rest8<T>(s[cc >> 1], pb, cc & 1), o[dt]);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[i], o[dt]);
             }
         }
     }

@@ -34,9 +34,6 @@ struct GradArgs {
 
 constexpr float kPShift = 8.0f;   // P is carried times 2^8
 
-// 1 - tanh^2 from the w of the score map.
-__device__ __forceinline__ float cap_slope(float w, int wide) { return wide ? 1.0f - w * w : -4.0f * w * (1.0f + w); }
-
 // The power of two that takes `most` to 2^-12 .. 2^-11 (with P's 2^8: 2^-4 .. 2^-3).
 __device__ __forceinline__ float scale_of(float most) {
     const int e = min(max(__builtin_amdgcn_frexp_expf(most), -100), 100);
@@ -70,7 +67,7 @@ __device__ __forceinline__ void add_diagonals(const float16v& ds, float (&acc)[5
 
 // dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
+__global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -132,13 +129,13 @@ __global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
         if (lane == 0) a.most[h * a.n_b32 + c.b32 + (qw >> 5)] = most;
     }
     const int R = BIAS ? a.radius : 0;
-    float far_l = a.map.ab, far_r = a.map.ab;
+    float far_l = 0.0f, far_r = 0.0f;
     if constexpr (BIAS) {
         const float* b = a.bias + (long long)h * (2 * R + 1);
         for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
-            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]) + a.map.ab;
-        far_l += bias2_of(b[0]);
-        far_r += bias2_of(b[2 * R]);
+            tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
+        far_l = bias2_of(b[0]);
+        far_r = bias2_of(b[2 * R]);
     }
     // the bias's gradient: a ring of 128 distances for each 16 lanes, see flush
     float* ring = tab + 2 * R + 1 + 2 * kTabPad + (3 - (2 * R + 2 * kTabPad) % 4) + wave * 512;
@@ -205,6 +202,7 @@ __global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
                 for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, add));
             }
             if (kb + kKeys > kfull) {
+                keep_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (kb + 32 * kt + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) ds[r] = 0.0f;
@@ -229,7 +227,7 @@ __global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
             }
             if constexpr (CAP) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] *= cap_slope(s[r], a.map.wide);
+                for (int r = 0; r < 16; ++r) ds[r] *= __builtin_fmaf(-s[r], s[r], 1.0f);
             }
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
@@ -279,11 +277,11 @@ __global__ __launch_bounds__(256) void relpos_dq_kernel(GradArgs a) {
 // dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 queries a step
 // through LDS, the heads that share the keys one after the other.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void relpos_dkv_kernel(GradArgs a) {
+__global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: ab - L2 and -delta sc of a step's queries
+    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 and -delta sc of a step's queries
     float* tab = rows + 256;
     const int id = xcd_swizzle(blockIdx.x, gridDim.x);
     const int kvh = id / a.n_tiles;
@@ -326,7 +324,7 @@ __global__ __launch_bounds__(256) void relpos_dkv_kernel(GradArgs a) {
             const long long at = h * a.total_q + c.q0 + min(qi, c.nq - 1);
             if (threadIdx.x < 64) {
                 const float lse = a.lse[at];
-                row_v = qi < c.nq && !(lse < -1e30f) ? a.map.ab + kPShift - lse * kLog2e : -FLT_MAX;
+                row_v = qi < c.nq && !(lse < -1e30f) ? kPShift - lse * kLog2e : -FLT_MAX;
             } else {
                 row_v = qi < c.nq ? -a.delta[at] * step_scale(h, q) : 0.0f;
             }
@@ -408,6 +406,7 @@ __global__ __launch_bounds__(256) void relpos_dkv_kernel(GradArgs a) {
                 for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, pr[r]));
             }
             if (a.causal && kw + 31 >= max(c.prefix, past + qs + 1)) {
+                keep_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (ki >= max(c.prefix, past + qs + 8 * (r >> 2) + 4 * hl + (r & 3) + 1)) pr[r] = 0.0f;
@@ -421,7 +420,7 @@ __global__ __launch_bounds__(256) void relpos_dkv_kernel(GradArgs a) {
             }
             if constexpr (CAP) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] *= cap_slope(s[r], a.map.wide);
+                for (int r = 0; r < 16; ++r) ds[r] *= __builtin_fmaf(-s[r], s[r], 1.0f);
             }
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
