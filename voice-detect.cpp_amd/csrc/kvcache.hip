@@ -133,7 +133,7 @@ struct PagedArgs {
     const int *table, *lens;
     int max_pages, max_len, n_heads, group, head_parts, splits, chunk;
     const float* bias;
-    int radius;
+    int radius, span;   // span: keys of a part that may have a bias of their own
     ScoreMap map;
     void* o;
     long long o_seq, o_head;
@@ -154,23 +154,25 @@ __device__ __forceinline__ typename Vec8<T>::type codes8(uint32_t lo, uint32_t h
     typename Vec8<T>::type v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float2v f = from_e4m3(j < 2 ? lo : hi, j & 1);
-        const auto p = pack2<T>(f[0], f[1]);
+        const uint32_t w = j < 2 ? lo : hi;
+        typename Vec8<T>::pair p;
+        if constexpr (std::is_same_v<T, half_t>)
+            p = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                      : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        else
+            p = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                      : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
         v[2 * j] = p[0];
         v[2 * j + 1] = p[1];
     }
     return v;
 }
 
-// DMA of BYTES a lane from per-lane addresses to LDS lds_dst + BYTES * lane
+// DMA of 4 bytes a lane from per-lane addresses to LDS lds_dst + 4 * lane
 // (lds_dst wave-uniform); ordered by the caller's vmcnt waits.
-template <int BYTES>
-__device__ __forceinline__ void dma_lanes(uint8_t* lds_dst, const void* src) {
+__device__ __forceinline__ void dma4_lanes(uint8_t* lds_dst, const void* src) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)lds_dst);
-    if constexpr (BYTES == 16)
-        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
-    else
-        asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
 }
 
 // 16-byte chunk c of ring row r: rows of RB bytes, swizzled so that the column
@@ -193,11 +195,12 @@ struct PagedShape {
 };
 
 template <class T, int D, bool QUANT, bool CAP>
-__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(PagedArgs a) {
     using S = PagedShape<T, D, QUANT>;
     using V8 = typename Vec8<T>::type;
     using PT = std::conditional_t<QUANT, bf16_t, T>;   // p times a value's scale may leave the range of f16
     using P8 = typename Vec8<PT>::type;
+    constexpr bool kTwo = QUANT && std::is_same_v<T, half_t>;   // then it takes two bf16 to keep f16's bits
     constexpr int kRow = S::kRow, kChunks = kRow / 16;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     int* pages = reinterpret_cast<int*>(smem + S::kLds);
@@ -211,47 +214,90 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
         atomicOr(a.status, VDK_STATUS_BAD_LENGTH);
     const int k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     if (k0 >= k1 && split > 0) return;
-    // the part's pages; -1 for one outside the cache
-    const int p0 = k0 >> a.page_shift, np = k1 > k0 ? ((k1 - 1) >> a.page_shift) - p0 + 1 : 0;
-    for (int i = threadIdx.x; i < np; i += 64 * kWaves) {
-        int p = a.table[(long long)seq * a.max_pages + p0 + i];
-        if (p < 0 || p >= a.n_pages) {
-            p = -1;
-            if (a.status) atomicOr(a.status, VDK_STATUS_BAD_PAGE);
-        }
-        pages[i] = p;
-    }
     const int hq = part * 16 + n16, head = kvh * a.group + min(hq, a.group - 1);
     const T* qp = static_cast<const T*>(a.q) + seq * a.q_seq + head * a.q_head;
     V8 qf[D / 32];   // slot (g, j) of product kk: e4m3 dims 64 (kk / 2) + 16 g + 8 (kk % 2) + j, else 32 kk + 8 g + j
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
         qf[kk] = *reinterpret_cast<const V8*>(qp + (QUANT ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
-    const float* bias = a.bias ? a.bias + (long long)head * (2 * a.radius + 1) : nullptr;
-    __syncthreads();
+    // the part's pages; -1 for one outside the cache
+    const int p0 = k0 >> a.page_shift, np = k1 > k0 ? ((k1 - 1) >> a.page_shift) - p0 + 1 : 0;
+    int bad = 0;
+    for (int i = threadIdx.x; i < np; i += 64 * kWaves) {
+        int p = a.table[(long long)seq * a.max_pages + p0 + i];
+        if (p < 0 || p >= a.n_pages) {
+            p = -1;
+            bad = 1;
+            if (a.status) atomicOr(a.status, VDK_STATUS_BAD_PAGE);
+        }
+        pages[i] = p;
+    }
+    // the bias of the keys from kn on; all before them share the head's first
+    const int heads = min(a.group - part * 16, 16);
+    int kn = a.bias ? max(k0, len - a.radius) : k1;
+    if (kn >= k1) kn = 1 << 30;   // none here
+    float* tab = reinterpret_cast<float*>(pages + (a.chunk >> a.page_shift));
+    float far = 0.0f;
+    if (a.bias) {
+        const float* b = a.bias + (long long)(kvh * a.group + part * 16) * (2 * a.radius + 1);
+        far = bias2_of(b[(long long)min(n16, heads - 1) * (2 * a.radius + 1)]);
+        for (int h = 0; h < heads; ++h)
+            for (int i = kn + (int)threadIdx.x; i < k1; i += 64 * kWaves)
+                tab[h * a.span + i - kn] = bias2_of(b[(long long)h * (2 * a.radius + 1) + i - (len - 1) + a.radius]);
+    }
+    tab += min(n16, heads - 1) * a.span;
+    bad = __syncthreads_or(bad);
+    // (the loop's waits count DMAs: no load of the compiler's may be open in it)
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) asm volatile("" : "+v"(qf[kk]));
+    asm volatile("" : "+v"(far));
 
     uint8_t* ring = smem + wave * S::kDepth * S::kStage;
-    auto row_of = [&](int key) {   // the cache row of a key (clamped into the part), its page -1: row 0 (hidden later)
-        const int k = min(key, k1 - 1), p = max(pages[(k >> a.page_shift) - p0], 0);
-        return (((long long)p * a.kv + kvh) << a.page_shift) + (k & (page - 1));
-    };
-    auto fetch = [&](int kb, int st) {
-        uint8_t* dst = ring + st * S::kStage;
+    const float* scales = QUANT ? (lane < 32 ? a.k_scale : a.v_scale) + (lane & 15) : nullptr;
+    uint32_t voff[16 * kRow / 1024];
 #pragma unroll
-        for (int j = 0; j < S::kTile / 1024; ++j) {
-            const int i = j * 64 + lane, r = i / kChunks, c = ring_chunk<kRow>(r, i % kChunks);
-            const long long at = row_of(kb + r) * kRow + 16 * c;
-            dma_lanes<16>(dst + j * 1024, a.k + at);
-            dma_lanes<16>(dst + S::kTile + j * 1024, a.v + at);
+    for (int j = 0; j < 16 * kRow / 1024; ++j) {
+        const int i = j * 64 + lane, r = i / kChunks;
+        voff[j] = r * kRow + 16 * ring_chunk<kRow>(r, i % kChunks);
+    }
+    // 16 keys lie in one page: its address is the wave's, and rows past the part or of a bad page read as zero
+    auto page_of = [&](int key) { return pages[(min(key, k1 - 1) >> a.page_shift) - p0]; };
+    auto fetch = [&](int kb, int st, int pg0, int pg1) {
+        uint8_t* dst = ring + st * S::kStage;
+        long long rows[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int pg = __builtin_amdgcn_readfirstlane(t ? pg1 : pg0), key = kb + 16 * t;
+            rows[t] = (((long long)max(pg, 0) * a.kv + kvh) << a.page_shift) + (key & (page - 1));
+            const int left = k1 - key, n = pg < 0 || left <= 0 ? 0 : left < 16 ? left : 16;
+            const uint32_t bytes = n * kRow;
+            const int4v rk = dma_rsrc(a.k + rows[t] * kRow, bytes), rv = dma_rsrc(a.v + rows[t] * kRow, bytes);
+            // five wait states between a vector write of a scalar (readfirstlane) and a buffer instruction that
+            // reads it, which the compiler does not count for instructions in inline assembly
+            asm volatile("s_nop 4" ::"s"(rk), "s"(rv));
+#pragma unroll
+            for (int j = 0; j < 16 * kRow / 1024; ++j) {
+                dma16(dst + t * 16 * kRow + j * 1024, rk, voff[j]);
+                dma16(dst + S::kTile + t * 16 * kRow + j * 1024, rv, voff[j]);
+            }
         }
-        if constexpr (QUANT)   // lanes 0..31: the keys' scales, 32..63: the values'
-            dma_lanes<4>(dst + 2 * S::kTile, (lane < 32 ? a.k_scale : a.v_scale) + row_of(kb + (lane & 31)));
+        // lanes 0 .. 31: the keys' scales, 32 .. 63: the values' (past the part: some row of a page, not used)
+        if constexpr (QUANT) dma4_lanes(dst + 2 * S::kTile, scales + (lane & 16 ? rows[1] : rows[0]));
     };
     const int first = k0 + wave * kStep;
     const int steps = first < k1 ? (k1 - first + kWaves * kStep - 1) / (kWaves * kStep) : 0;
 #pragma unroll
     for (int st = 0; st < S::kDepth - 1; ++st)
-        if (st < steps) fetch(first + st * kWaves * kStep, st);
+        if (st < steps) {
+            const int kb = first + st * kWaves * kStep;
+            fetch(kb, st, page_of(kb), page_of(kb + 16));
+        }
+    int pg0 = 0, pg1 = 0;   // the pages of the next fetch
+    if (S::kDepth - 1 < steps) {
+        const int kb = first + (S::kDepth - 1) * kWaves * kStep;
+        pg0 = page_of(kb);
+        pg1 = page_of(kb + 16);
+    }
 
     float4v o[D / 16];
 #pragma unroll
@@ -262,7 +308,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
         const int kb = first + it * kWaves * kStep;
         __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the stage to be filled is no longer read
         if (it + S::kDepth - 1 < steps) {
-            fetch(kb + (S::kDepth - 1) * kWaves * kStep, st == 0 ? S::kDepth - 1 : st - 1);
+            fetch(kb + (S::kDepth - 1) * kWaves * kStep, st == 0 ? S::kDepth - 1 : st - 1, pg0, pg1);
+            pg0 = page_of(kb + S::kDepth * kWaves * kStep);
+            pg1 = page_of(kb + S::kDepth * kWaves * kStep + 16);
             wait_vmcnt<(S::kDepth - 1) * S::kOps>();
         } else {
             wait_vmcnt<0>();
@@ -273,8 +321,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
         const float* sc = reinterpret_cast<const float*>(sk + 2 * S::kTile);
         // s[t][r]: key kb + 16 t + 4 g + r, head n16
         float4v s[2];
-        float mx = -INFINITY;
-        bool there[2];   // whether the 16 keys' page exists
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             s[t] = float4v{0, 0, 0, 0};
@@ -286,31 +332,42 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
                     s[t] = mfma16(codes8<T>(w[0], w[1]), qf[2 * i], s[t]);
                     s[t] = mfma16(codes8<T>(w[2], w[3]), qf[2 * i + 1], s[t]);
                 }
+                s[t] *= *reinterpret_cast<const float4v*>(sc + 16 * t + 4 * g);
             } else {
 #pragma unroll
                 for (int kk = 0; kk < D / 32; ++kk)
                     s[t] = mfma16(*reinterpret_cast<const V8*>(sk + row * kRow + 16 * ring_chunk<kRow>(row, 4 * kk + g)),
                                   qf[kk], s[t]);
             }
-            if constexpr (QUANT) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] *= sc[16 * t + 4 * g + r];
-            }
             score_w<CAP>(s[t], a.map);
             const int kt = kb + 16 * t + 4 * g;
-            there[t] = pages[(min(kb + 16 * t, k1 - 1) >> a.page_shift) - p0] >= 0;
+            if (kb + kStep > kn) {
+                keep_branch();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = min(max(kt + r - (len - 1), -a.radius), 0) + a.radius;   // (keys past the last: hidden)
-                const float b2 = bias ? bias2_of(bias[d]) : 0.0f;
-                const float w = __builtin_fmaf(s[t][r], a.map.am, b2);
-                s[t][r] = there[t] && kt + r < k1 ? w : -INFINITY;
-                mx = fmaxf(mx, s[t][r]);
+                for (int r = 0; r < 4; ++r) {
+                    const float b2 = tab[min(max(kt + r, kn), k1 - 1) - kn];
+                    s[t][r] = __builtin_fmaf(s[t][r], a.map.am, kt + r >= kn ? b2 : far);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][r] = __builtin_fmaf(s[t][r], a.map.am, far);
+            }
+            if (bad || kb + kStep > k1) {
+                keep_branch();
+                const bool there = page_of(kb + 16 * t) >= 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!there || kt + r >= k1) s[t][r] = -INFINITY;
             }
         }
+        float mx = max3(s[0][0], s[0][1], s[0][2]);
+        mx = max3(mx, s[0][3], s[1][0]);
+        mx = max3(mx, s[1][1], s[1][2]);
+        mx = fmaxf(mx, s[1][3]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         if (__any(mx > m + 8.0f)) {
+            keep_branch();
             const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
             l *= alpha;
@@ -319,16 +376,30 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
         }
         P8 hi, lo;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            float p[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float p = __builtin_amdgcn_exp2f(s[t][r] - m);
-                l += p;
-                if constexpr (QUANT) p = s[t][r] == -INFINITY ? 0.0f : p * sc[32 + 16 * t + 4 * g + r];
-                hi[4 * t + r] = (PT)p;
-                // half type: p in two bf16 parts, 16 bits of it together
-                if constexpr (QUANT) lo[4 * t + r] = (PT)(p - (float)hi[4 * t + r]);
+                p[r] = __builtin_amdgcn_exp2f(s[t][r] - m);
+                l += p[r];
             }
+            if constexpr (QUANT) {
+                const float4v vs = *reinterpret_cast<const float4v*>(sc + 32 + 16 * t + 4 * g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = p[r] == 0.0f ? 0.0f : p[r] * vs[r];   // (a hidden row's scale may be anything)
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                const auto h2 = pack2<PT>(p[r], p[r + 1]);
+                hi[4 * t + r] = h2[0];
+                hi[4 * t + r + 1] = h2[1];
+                if constexpr (kTwo) {   // p in two bf16 parts, 16 bits of it
+                    const auto l2 = pack2<PT>(p[r] - (float)h2[0], p[r + 1] - (float)h2[1]);
+                    lo[4 * t + r] = l2[0];
+                    lo[4 * t + r + 1] = l2[1];
+                }
+            }
+        }
         // V^T: row (dim) n16 of tile dt, slots the keys 4 g + {0..3} and 16 + 4 g + {0..3}
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) {
@@ -336,17 +407,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
                 const int j = n16 >> 1, row = 16 * (j >> 2) + 4 * g + (j & 3);
                 const uint8_t* p = sv + row * kRow + 16 * ring_chunk<kRow>(row, dt) + 8 * (n16 & 1);
                 const int2v w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2v*)p);
-                const P8 va = codes8<PT>(there[0] ? w[0] : 0, there[1] ? w[1] : 0);
+                const P8 va = codes8<PT>(w[0], w[1]);
                 o[dt] = mfma16(va, hi, o[dt]);
-                if constexpr (std::is_same_v<T, half_t>) o[dt] = mfma16(va, lo, o[dt]);
+                if constexpr (kTwo) o[dt] = mfma16(va, lo, o[dt]);
             } else {
                 const int r0 = 4 * g + (n16 >> 2), r1 = 16 + r0, c = 2 * dt + ((n16 & 3) >> 1), e = 8 * (n16 & 1);
                 const short4v x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (lds_short4v*)(sv + r0 * kRow + 16 * ring_chunk<kRow>(r0, c) + e));
                 const short4v x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (lds_short4v*)(sv + r1 * kRow + 16 * ring_chunk<kRow>(r1, c) + e));
-                const short4v none = {0, 0, 0, 0}, y0 = there[0] ? x0 : none, y1 = there[1] ? x1 : none;
-                o[dt] = mfma16(__builtin_bit_cast(P8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7)), hi, o[dt]);
+                o[dt] = mfma16(__builtin_bit_cast(P8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7)), hi, o[dt]);
             }
         }
     }
@@ -364,7 +434,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(PagedArgs a) {
         mine[D + 1] = l;
     }
     __syncthreads();
-    const int heads = min(a.group - part * 16, 16);
     for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kWaves) {
         const int hh = i / (D / 4), d = 4 * (i % (D / 4));
         const float* p = js + hh * kJ;
@@ -484,14 +553,17 @@ int cache_rows(const vdk_kv_cache* c, const long long* slots, long long n, void*
 
 // How many parts a stream's keys are cut into, and how long one is.
 struct Cut {
-    int splits, chunk;
+    int splits, chunk, span;
 };
 Cut cut_of(const vdk_kv_cache* c, const vdk_paged_attn* a) {
     const long long groups = (long long)a->n_seqs * c->n_kv_heads * cdiv(a->n_q_heads / c->n_kv_heads, 16);
     const long long want = std::max(1ll, 2048 / std::max(groups, 1ll));
     long long chunk = (a->max_len + want - 1) / want;
     chunk = std::min(std::max((chunk + 127) / 128 * 128, 512ll), 8192ll);
-    return {(int)std::max(1ll, (a->max_len + chunk - 1) / chunk), (int)chunk};
+    // a part's biases stay in LDS: 24 KB of them
+    const long long most = 6144 / std::min(a->n_q_heads / c->n_kv_heads, 16), near = a->dist_bias ? a->bias_radius : 0;
+    if (near > most) chunk = std::min(chunk, most / 128 * 128);
+    return {(int)std::max(1ll, (a->max_len + chunk - 1) / chunk), (int)chunk, (int)std::min(chunk, near)};
 }
 
 void check_paged(const vdk_kv_cache* c, const vdk_paged_attn* a) {
@@ -508,7 +580,7 @@ void check_paged(const vdk_kv_cache* c, const vdk_paged_attn* a) {
 template <class T, int D, bool QUANT, bool CAP>
 void launch_paged(PagedArgs a, int n_seqs, hipStream_t s) {
     auto kern = paged_attn_kernel<T, D, QUANT, CAP>;
-    const int lds = PagedShape<T, D, QUANT>::kLds + 4 * ((a.chunk >> a.page_shift) + 2);
+    const int lds = PagedShape<T, D, QUANT>::kLds + 4 * (a.chunk >> a.page_shift) + 4 * std::min(a.group, 16) * a.span;
     if (lds > 65536)
         VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     hipLaunchKernelGGL(kern, dim3((unsigned)n_seqs * a.kv * a.head_parts * a.splits), dim3(64 * kWaves), lds, s, a);
@@ -582,8 +654,8 @@ extern "C" int vdk_paged_attention(const vdk_kv_cache* c, const vdk_paged_attn* 
         PagedArgs p{static_cast<const uint8_t*>(c->k), static_cast<const uint8_t*>(c->v), c->k_scale, c->v_scale,
                     c->n_pages, shift_of(c->page_size), c->n_kv_heads, a->q, a->q_seq, a->q_head, a->block_table,
                     a->seq_lens, a->max_pages, a->max_len, a->n_q_heads, group, parts, cut.splits, cut.chunk,
-                    a->dist_bias, a->dist_bias ? a->bias_radius : 0, score_map(a->scale, a->cap), a->o, a->o_seq,
-                    a->o_head, a->lse, static_cast<float*>(a->work), a->status};
+                    a->dist_bias, a->dist_bias ? a->bias_radius : 0, cut.span, score_map(a->scale, a->cap), a->o,
+                    a->o_seq, a->o_head, a->lse, static_cast<float*>(a->work), a->status};
         hipStream_t s = static_cast<hipStream_t>(stream);
         const bool q = c->format == VDK_KV_E4M3, cap = a->cap > 0;
         if (c->dtype == VDK_F16)
