@@ -188,7 +188,7 @@ struct PagedShape {
     static constexpr int kTile = kStep * kRow;                       // keys (or values) of a step
     static constexpr int kStage = 2 * kTile + (QUANT ? 256 : 0);     // + 32 + 32 scales
     static constexpr int kOps = 2 * kTile / 1024 + (QUANT ? 1 : 0);  // DMA instructions of a stage
-    static constexpr int kDepth = kTile <= 4096 ? 3 : 2;
+    static constexpr int kDepth = 2;
     static constexpr int kRing = kWaves * kDepth * kStage;
     static constexpr int kJoin = kWaves * 16 * (D + 4) * 4;          // after the loop, in the ring's place
     static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
@@ -557,9 +557,9 @@ struct Cut {
 };
 Cut cut_of(const vdk_kv_cache* c, const vdk_paged_attn* a) {
     const long long groups = (long long)a->n_seqs * c->n_kv_heads * cdiv(a->n_q_heads / c->n_kv_heads, 16);
-    const long long want = std::max(1ll, 2048 / std::max(groups, 1ll));
-    long long chunk = (a->max_len + want - 1) / want;
-    chunk = std::min(std::max((chunk + 127) / 128 * 128, 512ll), 8192ll);
+    const long long least = std::min(std::max(2 * groups, 512ll), 2048ll);
+    long long chunk = a->max_len * groups / 2048;
+    chunk = std::min(std::max(chunk, least), 8192ll) / 128 * 128;
     // a part's biases stay in LDS: 24 KB of them
     const long long most = 6144 / std::min(a->n_q_heads / c->n_kv_heads, 16), near = a->dist_bias ? a->bias_radius : 0;
     if (near > most) chunk = std::min(chunk, most / 128 * 128);
