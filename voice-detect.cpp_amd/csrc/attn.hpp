@@ -87,6 +87,17 @@ __device__ __forceinline__ void keep_branch() { asm volatile("; rare"); }
 // The other 32 lanes' value.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
+// The largest of 32 registers, two chains.
+__device__ __forceinline__ float max32(const float16v& a, const float16v& b) {
+    float x = max3(a[0], a[1], a[2]), y = max3(b[0], b[1], b[2]);
+#pragma unroll
+    for (int r = 3; r < 15; r += 2) {
+        x = max3(x, a[r], a[r + 1]);
+        y = max3(y, b[r], b[r + 1]);
+    }
+    return fmaxf(max3(x, y, a[15]), b[15]);
+}
+
 // ---- LDS tiles of D 16-bit columns, dense rows ----
 // Row r's 16-byte chunk c lies at chunk position c ^ swz(r).  Sixteen rows'
 // same chunk (an A operand's read) then lie in sixteen different bank groups,
@@ -123,27 +134,44 @@ struct TileDma {
     }
 };
 
-// A operand rows row0 + lane % 32, columns 16 kk + 8 (lane / 32) .. + 7.
+// A lane's LDS addresses in such a tile, made once: a tile's place, a block of
+// rows and (for the transposing reads) of 16 rows are constants added by the
+// load instructions.
+//   row_block: A operand of rows 32 t + lane % 32, columns 16 kk + 8 (lane / 32) .. + 7.
+//   col_block: A operand of the transposed tile: its row is column 32 dt + lane %
+//     32 of the tile, its eight k-slots the rows 16 c + 4 h + {0..3} and 16 c + 8 +
+//     4 h + {0..3} (h = lane / 32).  Of each 16 lanes of a transposing read lane i
+//     supplies 8 bytes of row i / 4 and receives column i of the four rows.
 template <class T, int D>
-__device__ __forceinline__ typename Vec8<T>::type tile_rows(const uint8_t* lds, int row0, int kk, int lane) {
-    return *reinterpret_cast<const typename Vec8<T>::type*>(
-        lds + tile_at<D>(row0 + (lane & 31), 2 * kk + (lane >> 5)));
-}
-
-// A operand of the transposed tile: row (of A) = column 32 dt + lane % 32 of
-// the tile, its eight k-slots the tile's rows row0 + 4 h + {0..3} and row0 + 8
-// + 4 h + {0..3} (h = lane / 32).  Of each 16 lanes of a transposing read, lane
-// i supplies 8 bytes of row i / 4 and receives column i of the four rows.
-template <class T, int D>
-__device__ __forceinline__ typename Vec8<T>::type tr_pair(const uint8_t* lds, int row0, int dt, int lane) {
-    const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2);
-    const int col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-    const uint8_t* p0 = lds + tile_at<D>(row, col >> 3) + (col & 4) * 2;
-    const uint8_t* p1 = lds + tile_at<D>(row + 8, col >> 3) + (col & 4) * 2;
-    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p0);
-    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p1);
-    return __builtin_bit_cast(typename Vec8<T>::type, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-}
+struct TileReads {
+    using V8 = typename Vec8<T>::type;
+    uint32_t row[D / 16], col[D / 32][2];
+    __device__ __forceinline__ void init(const uint8_t* lds, int lane) {
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)lds;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            row[kk] = base + tile_at<D>(lane & 31, 2 * kk + (lane >> 5));
+            asm volatile("" : "+v"(row[kk]));   // kept, not made again in every step
+        }
+        const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+                col[dt][e] = base + tile_at<D>(r + 8 * e, c >> 3) + (c & 4) * 2;
+                asm volatile("" : "+v"(col[dt][e]));
+            }
+    }
+    __device__ __forceinline__ V8 row_block(int tile, int t, int kk) const {
+        return *(const __attribute__((address_space(3))) V8*)(uintptr_t)(row[kk] + tile + t * (64 * D));
+    }
+    __device__ __forceinline__ V8 col_block(int tile, int c, int dt) const {
+        const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(uintptr_t)(col[dt][0] + tile + c * (32 * D)));
+        const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(uintptr_t)(col[dt][1] + tile + c * (32 * D)));
+        return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
 
 // ---- scores ----
 // Scores are kept in units of log 2: s2 = am * w + bias2, with w = q . k without

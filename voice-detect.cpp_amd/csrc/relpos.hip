@@ -26,16 +26,17 @@ struct FwdArgs {
 
 // One workgroup: 32 NW queries of one head, wave w its rows 32 w ..; 64 keys a
 // step through double-buffered LDS tiles.  S^T = K Q^T leaves a query's scores
-// in one lane (pair), so the softmax needs no exchange inside the loop: the
-// row's running maximum moves only when it grows by more than 8 (p <= 2^8, and
-// 16-bit p keep their relative precision), and each lane sums its own keys.
+// in one lane (pair), so the softmax needs no exchange inside the loop: each
+// lane sums its own keys, and the row's reference m follows the maximum only
+// when a lane's sum of a tile passes 2^13 (p < 2^13 keep their precision in 16
+// bits, and the largest p of a row is 1 or more).
 // P^T then is the B operand of O^T += V^T P^T, V^T read by transposing LDS loads.
 // SPLIT (training, where o_f32 is wanted): P enters in 16-bit parts, two of f16
 // or three of bf16, 22 or 24 bits of it.  The backward pass takes delta = sum(o
 // dO) from o, and a bias's gradient sums dS over whole rows, where its terms
 // cancel and delta's error does not.
 template <class T, int D, int NW, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, 2) void relpos_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void relpos_fwd_kernel(FwdArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -85,21 +86,22 @@ __global__ __launch_bounds__(64 * NW, 2) void relpos_fwd_kernel(FwdArgs a) {
     float16v o[D / 32];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) o[dt] = splat16(0.0f);
+    TileReads<T, D> at;
+    at.init(smem, lane);
     float m = -FLT_MAX, l = 0.0f;
     const float am = a.map.am;
-    for (int kb = 0, buf = 0; kb < kend; kb += kKeys, buf ^= 1) {
+    auto step = [&](int kb, int buf) {
         wait_vmcnt<0>();
         lds_barrier();   // this tile is there, and the other buffer is no longer read
         if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
-        if (kb >= kend_w) continue;
-        const uint8_t* sk = smem + buf * 2 * kTile;
-        const uint8_t* sv = sk + kTile;
+        if (kb >= kend_w) return;
+        const int tk = buf * 2 * kTile, tv = tk + kTile;
         float16v s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             s[kt] = splat16(0.0f);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s[kt] = mfma32(tile_rows<T, D>(sk, 32 * kt, kk, lane), qf[kk], s[kt]);
+            for (int kk = 0; kk < D / 16; ++kk) s[kt] = mfma32(at.row_block(tk, kt, kk), qf[kk], s[kt]);
             score_w<CAP>(s[kt], a.map);
         }
         // s[kt][r]: key kb + 32 kt + 8 (r / 4) + 4 hl + r % 4 of query qi
@@ -132,15 +134,34 @@ __global__ __launch_bounds__(64 * NW, 2) void relpos_fwd_kernel(FwdArgs a) {
             mul = 1.0f;
             add = 0.0f;
         }
-        float mx = max3(s[0][0], s[0][1], s[1][0]);
+        // p = exp2(s2 - m) and its sum; only where a lane's sum passes 2^13 (as in the first tile) does the row's
+        // maximum move, and p is taken again: no maximum is looked for in the others
+        constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
+        V8 pb[4][kParts];
+        auto exponentials = [&] {
+            float sum[2] = {0.0f, 0.0f};
+            const float minus = add - m;
 #pragma unroll
-        for (int r = 2; r < 16; r += 2) mx = max3(mx, s[0][r], s[0][r + 1]);
+            for (int cc = 0; cc < 4; ++cc) {
+                float16v p;   // (eight of them, as pack8 takes them)
 #pragma unroll
-        for (int r = 1; r < 15; r += 2) mx = max3(mx, s[1][r], s[1][r + 1]);
-        mx = max3(mx, s[1][15], mx);
-        mx = __builtin_fmaf(fmaxf(mx, other_half(mx)), mul, add);
-        if (__any(mx > m + 8.0f)) {
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc >> 1][8 * (cc & 1) + j], mul, minus));
+                    sum[j & 1] += p[j];
+                }
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) {
+                    pb[cc][i] = pack8<T>(p, 0);
+                    if (i + 1 < kParts) take8<T>(p, pb[cc][i], 0);
+                }
+            }
+            return sum[0] + sum[1];
+        };
+        float sum = exponentials();
+        if (__any(!(sum < 8192.0f))) {
             keep_branch();
+            float mx = __builtin_fmaf(max32(s[0], s[1]), mul, add);
+            mx = fmaxf(mx, other_half(mx));
             const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
             l *= alpha;
@@ -148,32 +169,21 @@ __global__ __launch_bounds__(64 * NW, 2) void relpos_fwd_kernel(FwdArgs a) {
             for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+            sum = exponentials();
         }
-        add -= m;
+        l += sum;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], mul, add));
-                s[kt][r] = p;
-                l += p;
-            }
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-            constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
-            V8 pb[kParts];
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) {
-                pb[i] = pack8<T>(s[cc >> 1], cc & 1);
-                if (i + 1 < kParts) take8<T>(s[cc >> 1], pb[i], cc & 1);
-            }
+        for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt) {
-                const V8 vt = tr_pair<T, D>(sv, 16 * cc, dt, lane);
+                const V8 vt = at.col_block(tv, cc, dt);
 #pragma unroll
-                for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[i], o[dt]);
+                for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[cc][i], o[dt]);
             }
-        }
+    };
+    for (int kb = 0; kb < kend; kb += 2 * kKeys) {
+        step(kb, 0);
+        if (kb + kKeys < kend) step(kb + kKeys, 1);
     }
     if (qi >= c.nq) return;
     l += other_half(l);

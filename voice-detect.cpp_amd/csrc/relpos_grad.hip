@@ -172,14 +172,15 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) dq[dt] = splat16(0.0f);
     const float am = a.map.am;
+    TileReads<T, D> at;
+    at.init(smem, lane);
     const float unscale = kScaled<T> ? 1.0f / sc * 0x1p-8f : 1.0f;   // of dS, per row (a power of two)
     for (int kb = 0, buf = 0; kb < kend; kb += kKeys, buf ^= 1) {
         wait_vmcnt<0>();
         lds_barrier();
         if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
         if (kb >= kend_w) continue;
-        const uint8_t* sk = smem + buf * 2 * kTile;
-        const uint8_t* sv = sk + kTile;
+        const int tk = buf * 2 * kTile, tv = tk + kTile;
         const int d0 = kb - (qw + past);
         const bool near = BIAS && d0 + 63 > -R && d0 - 31 < R;
         const float add = (d0 < 0 ? far_l : far_r) - L2;
@@ -187,9 +188,9 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
         for (int kt = 0; kt < 2; ++kt) {
             float16v s = splat16(0.0f), p = splat16(0.0f);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(tile_rows<T, D>(sk, 32 * kt, kk, lane), qf[kk], s);
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tk, kt, kk), qf[kk], s);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(tile_rows<T, D>(sv, 32 * kt, kk, lane), df[kk], p);
+            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(tv, kt, kk), df[kk], p);
             score_w<CAP>(s, a.map);
             float16v ds;
             if (near) {
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
                 const V8 pb = pack8<T>(ds, cc);
 #pragma unroll
                 for (int dt = 0; dt < D / 32; ++dt)
-                    dq[dt] = mfma32(tr_pair<T, D>(sk, 32 * kt + 16 * cc, dt, lane), pb, dq[dt]);
+                    dq[dt] = mfma32(at.col_block(tk, 2 * kt + cc, dt), pb, dq[dt]);
             }
         }
         if constexpr (BIAS) {
@@ -337,6 +338,8 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = splat16(0.0f);
     const float am = a.map.am;
+    TileReads<T, D> at;
+    at.init(smem, lane);
     float sc = 0x1p-8f, far_l = 0.0f, far_r = 0.0f;
     if constexpr (kScaled<T>) {
         if (steps > 0) sc = step_scale(kvh * a.group, q_first);
@@ -370,17 +373,16 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
                 sc = s_new;
             }
         }
-        const uint8_t* sq = smem + buf * 2 * kTile;
-        const uint8_t* so = sq + kTile;
+        const int tq = buf * 2 * kTile, to = tq + kTile;
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) {
             const int qs = q + 32 * qt;
             if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
             float16v s = splat16(0.0f), p = splat16(0.0f);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(tile_rows<T, D>(sq, 32 * qt, kk, lane), kf[kk], s);
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kf[kk], s);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(tile_rows<T, D>(so, 32 * qt, kk, lane), vf[kk], p);
+            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(to, qt, kk), vf[kk], p);
             score_w<CAP>(s, a.map);
             // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki
             const int d0 = kw - (qs + past);   // distances d0 - 31 .. d0 + 31
@@ -427,8 +429,8 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
                 const V8 pb = pack8<T>(pr, cc), db = pack8<T>(ds, cc);
 #pragma unroll
                 for (int dt = 0; dt < D / 32; ++dt) {
-                    dv[dt] = mfma32(tr_pair<T, D>(so, 32 * qt + 16 * cc, dt, lane), pb, dv[dt]);
-                    dk[dt] = mfma32(tr_pair<T, D>(sq, 32 * qt + 16 * cc, dt, lane), db, dk[dt]);
+                    dv[dt] = mfma32(at.col_block(to, 2 * qt + cc, dt), pb, dv[dt]);
+                    dk[dt] = mfma32(at.col_block(tq, 2 * qt + cc, dt), db, dk[dt]);
                 }
             }
         }
