@@ -87,15 +87,12 @@ __device__ __forceinline__ void keep_branch() { asm volatile("; rare"); }
 // The other 32 lanes' value.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-// The largest of 32 registers, two chains.
-__device__ __forceinline__ float max32(const float16v& a, const float16v& b) {
-    float x = max3(a[0], a[1], a[2]), y = max3(b[0], b[1], b[2]);
+// The largest of 16 registers.
+__device__ __forceinline__ float max16(const float16v& a) {
+    float x = max3(a[0], a[1], a[2]);
 #pragma unroll
-    for (int r = 3; r < 15; r += 2) {
-        x = max3(x, a[r], a[r + 1]);
-        y = max3(y, b[r], b[r + 1]);
-    }
-    return fmaxf(max3(x, y, a[15]), b[15]);
+    for (int r = 3; r < 15; r += 2) x = max3(x, a[r], a[r + 1]);
+    return fmaxf(x, a[15]);
 }
 
 // ---- LDS tiles of D 16-bit columns, dense rows ----

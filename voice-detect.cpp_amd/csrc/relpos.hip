@@ -36,7 +36,7 @@ struct FwdArgs {
 // dO) from o, and a bias's gradient sums dS over whole rows, where its terms
 // cancel and delta's error does not.
 template <class T, int D, int NW, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void relpos_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(FwdArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -96,90 +96,84 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void relpos_fwd_kernel(Fw
         if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
         if (kb >= kend_w) return;
         const int tk = buf * 2 * kTile, tv = tk + kTile;
-        float16v s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            s[kt] = splat16(0.0f);
+            const int k0 = kb + 32 * kt;
+            if (kt && k0 >= kend_w) break;
+            float16v s = splat16(0.0f);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s[kt] = mfma32(at.row_block(tk, kt, kk), qf[kk], s[kt]);
-            score_w<CAP>(s[kt], a.map);
-        }
-        // s[kt][r]: key kb + 32 kt + 8 (r / 4) + 4 hl + r % 4 of query qi
-        if (kb + kKeys > kfull) {
-            keep_branch();
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (kb + 32 * kt + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) s[kt][r] = -INFINITY;
-        }
-        const int d0 = kb - (qw + past);   // distances of the tile: d0 - 31 .. d0 + 63
-        const bool near = R != 0 && d0 + 63 > -R && d0 - 31 < R;
-        float mul = am, add = d0 < 0 ? far_l : far_r;
-        if (near) {
-            const float* t = tab + (d0 - lr + 4 * hl + R + kTabPad);
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tk, kt, kk), qf[kk], s);
+            score_w<CAP>(s, a.map);
+            // s[r]: key k0 + 8 (r / 4) + 4 hl + r % 4 of query qi
+            if (k0 + 32 > kfull) {
+                keep_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[kt][r] = __builtin_fmaf(s[kt][r], am, t[32 * kt + 8 * (r >> 2) + (r & 3)]);
-            mul = 1.0f;
-            add = 0.0f;
-        } else if (add < -1e37f) {   // a far bias of the lowest value takes the products in, as the near ones do
-            keep_branch();
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_fmaf(s[kt][r], am, add);
-            mul = 1.0f;
-            add = 0.0f;
-        }
-        // p = exp2(s2 - m) and its sum; only where a lane's sum passes 2^13 (as in the first tile) does the row's
-        // maximum move, and p is taken again: no maximum is looked for in the others
-        constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
-        V8 pb[4][kParts];
-        auto exponentials = [&] {
-            float sum[2] = {0.0f, 0.0f};
-            const float minus = add - m;
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) {
-                float16v p;   // (eight of them, as pack8 takes them)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc >> 1][8 * (cc & 1) + j], mul, minus));
-                    sum[j & 1] += p[j];
-                }
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) {
-                    pb[cc][i] = pack8<T>(p, 0);
-                    if (i + 1 < kParts) take8<T>(p, pb[cc][i], 0);
-                }
+                    if (k0 + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) s[r] = -INFINITY;
             }
-            return sum[0] + sum[1];
-        };
-        float sum = exponentials();
-        if (__any(!(sum < 8192.0f))) {
-            keep_branch();
-            float mx = __builtin_fmaf(max32(s[0], s[1]), mul, add);
-            mx = fmaxf(mx, other_half(mx));
-            const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            l *= alpha;
+            const int d0 = k0 - (qw + past);   // distances of the block: d0 - 31 .. d0 + 31
+            const bool near = R != 0 && d0 + 31 > -R && d0 - 31 < R;
+            float mul = am, add = d0 < 0 ? far_l : far_r;
+            if (near) {
+                const float* t = tab + (d0 - lr + 4 * hl + R + kTabPad);
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], am, t[8 * (r >> 2) + (r & 3)]);
+                mul = 1.0f;
+                add = 0.0f;
+            } else if (add < -1e37f) {   // a far bias of the lowest value takes the products in, as the near ones do
+                keep_branch();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-            sum = exponentials();
-        }
-        l += sum;
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt) {
-                const V8 vt = at.col_block(tv, cc, dt);
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[cc][i], o[dt]);
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], am, add);
+                mul = 1.0f;
+                add = 0.0f;
             }
+            // p = exp2(s2 - m) and its sum; only where a lane's sum passes 2^13 (as in the first block) does the row's
+            // maximum move, and p is taken again: no maximum is looked for in the others
+            constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
+            V8 pb[2][kParts];
+            auto exponentials = [&] {
+                float sum[2] = {0.0f, 0.0f};
+                const float minus = add - m;
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    float16v p;   // (eight of them, as pack8 takes them)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * cc + j], mul, minus));
+                        sum[j & 1] += p[j];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) {
+                        pb[cc][i] = pack8<T>(p, 0);
+                        if (i + 1 < kParts) take8<T>(p, pb[cc][i], 0);
+                    }
+                }
+                return sum[0] + sum[1];
+            };
+            float sum = exponentials();
+            if (__any(!(sum < 8192.0f))) {
+                keep_branch();
+                float mx = __builtin_fmaf(max16(s), mul, add);
+                mx = fmaxf(mx, other_half(mx));
+                const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+                sum = exponentials();
+            }
+            l += sum;
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt) {
+                    const V8 vt = at.col_block(tv, 2 * kt + cc, dt);
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[cc][i], o[dt]);
+                }
+        }
     };
     for (int kb = 0; kb < kend; kb += 2 * kKeys) {
         step(kb, 0);

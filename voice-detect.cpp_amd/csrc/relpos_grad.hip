@@ -10,6 +10,8 @@
 // P is carried times 2^8 and, in f16, dx times a power of two that brings the
 // row's (block's) largest |dO| to 2^-4 .. 2^-3: both are rounded to 16 bits as
 // MFMA operands, and the powers keep them clear of f16's subnormal numbers.
+#include <algorithm>
+
 #include "attn.hpp"
 
 namespace vdk {
@@ -29,7 +31,9 @@ struct GradArgs {
     const AttnClip* clips;
     const int2* tiles;
     int n_tiles, n_heads, n_kv, group, causal, n_b32;
-    long long total_q;
+    long long total_q, total_kv;
+    float* kv_part;                        // [head_parts][2][total_kv][n_kv][D], where the heads of a key head are split
+    int head_parts;
 };
 
 constexpr float kPShift = 8.0f;   // P is carried times 2^8
@@ -276,7 +280,8 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
 }
 
 // dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 queries a step
-// through LDS, the heads that share the keys one after the other.
+// through LDS, the heads that share the keys one after the other, or a part of
+// them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
 template <class T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     using V8 = typename Vec8<T>::type;
@@ -285,8 +290,9 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 and -delta sc of a step's queries
     float* tab = rows + 256;
     const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-    const int kvh = id / a.n_tiles;
-    const int2 tile = a.tiles[id - kvh * a.n_tiles];
+    const int of = id / a.n_tiles, kvh = of / a.head_parts, hp = of - kvh * a.head_parts;
+    const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
+    const int2 tile = a.tiles[id - of * a.n_tiles];
     const AttnClip c = a.clips[tile.x];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
@@ -294,7 +300,7 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     const int kr = ki < c.nk ? ki : c.nk - 1;
     // the first query that sees a key of the tile, down to a whole step
     const int q_first = a.causal && tile.y >= c.prefix ? max(tile.y - past, 0) & ~63 : 0;
-    const int per_head = q_first < c.nq ? (c.nq - q_first + 63) >> 6 : 0, steps = per_head * a.group;
+    const int per_head = q_first < c.nq ? (c.nq - q_first + 63) >> 6 : 0, steps = per_head * heads;
 
     const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + (c.k0 + kr) * a.v_tok + (long long)kvh * a.v_head;
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
         return scale_of(q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
     };
     auto fetch = [&](int it, int buf) {
-        const int h = kvh * a.group + it / per_head, q = q_first + (it % per_head) * 64;
+        const int h = h0 + it / per_head, q = q_first + (it % per_head) * 64;
         const T* qs = static_cast<const T*>(a.q) + (c.q0 + q) * a.q_tok + (long long)h * a.q_head;
         const T* ds = static_cast<const T*>(a.d_o) + (c.q0 + q) * a.do_tok + (long long)h * a.do_head;
         dmq.load(smem + buf * 2 * kTile, qs, qb_row, c.nq - q, wave);
@@ -342,10 +348,10 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     at.init(smem, lane);
     float sc = 0x1p-8f, far_l = 0.0f, far_r = 0.0f;
     if constexpr (kScaled<T>) {
-        if (steps > 0) sc = step_scale(kvh * a.group, q_first);
+        if (steps > 0) sc = step_scale(h0, q_first);
     }
     for (int it = 0, buf = 0; it < steps; ++it, buf ^= 1) {
-        const int hg = it / per_head, h = kvh * a.group + hg, q = q_first + (it % per_head) * 64;
+        const int h = h0 + it / per_head, q = q_first + (it % per_head) * 64;
         if constexpr (BIAS) {
             if (it % per_head == 0) {   // another head's bias
                 lds_barrier();
@@ -437,6 +443,24 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
     }
     if (ki >= c.nk) return;
     const float f = a.scale * 0x1p-8f / sc;
+    if (a.head_parts > 1) {
+        float* out = a.kv_part + (((long long)hp * 2 * a.total_kv + c.k0 + ki) * a.n_kv + kvh) * D;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float4v k4, v4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    k4[e] = dk[dt][4 * g + e] * f;
+                    v4[e] = dv[dt][4 * g + e] * 0x1p-8f;
+                }
+                float* at = out + 32 * dt + 8 * g + 4 * hl;
+                *reinterpret_cast<float4v*>(at) = k4;
+                *reinterpret_cast<float4v*>(at + a.total_kv * a.n_kv * D) = v4;
+            }
+        return;
+    }
     T* ok = static_cast<T*>(a.dk) + (c.k0 + ki) * a.dk_tok + (long long)kvh * a.dk_head;
     T* ov = static_cast<T*>(a.dv) + (c.k0 + ki) * a.dv_tok + (long long)kvh * a.dv_head;
 #pragma unroll
@@ -452,6 +476,38 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
             put(ok, dk[dt], f);
             put(ov, dv[dt], 0x1p-8f);
         }
+}
+
+// The parts of relpos_dkv_kernel added up, 8 values a thread.
+template <class T, int D>
+__global__ __launch_bounds__(256) void relpos_dkv_join_kernel(GradArgs a) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / (D / 8);
+    const int d = 8 * (int)(i % (D / 8));
+    if (row >= a.total_kv * a.n_kv) return;
+    const long long tok = row / a.n_kv, size = a.total_kv * a.n_kv * D;
+    const int h = (int)(row - tok * a.n_kv);
+    const float* p = a.kv_part + blockIdx.y * size + row * D + d;
+    float4v s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+    for (int j = 0; j < a.head_parts; ++j, p += 2 * size) {
+        s0 += *reinterpret_cast<const float4v*>(p);
+        s1 += *reinterpret_cast<const float4v*>(p + 4);
+    }
+    T* out = blockIdx.y ? static_cast<T*>(a.dv) + tok * a.dv_tok + h * a.dv_head
+                        : static_cast<T*>(a.dk) + tok * a.dk_tok + h * a.dk_head;
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = (T)s0[e];
+        v[4 + e] = (T)s1[e];
+    }
+    *reinterpret_cast<typename Vec8<T>::type*>(out + d) = v;
+}
+
+// How many parts the heads of a key head are cut into: 1024 workgroups fill the
+// chip twice, and causal tiles differ most in their work where they are few.
+int head_parts_of(const vdk_attn_plan* p) {
+    const long long groups = std::max(1ll, (long long)p->n_k128 * p->n_kv);
+    return (int)std::max(1ll, std::min<long long>(p->n_heads / p->n_kv, (1024 + groups - 1) / groups));
 }
 
 // The blocks' partial sums of 64 distances, 16 rows of blocks at a time, in a fixed order.
@@ -499,8 +555,13 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
             VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         a.tiles = p->d_k128;
         a.n_tiles = p->n_k128;
-        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_kv), dim3(256), lds, s, a);
+        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_kv * a.head_parts), dim3(256), lds, s, a);
         VDK_HIP(hipGetLastError());
+        if (a.head_parts > 1) {
+            const long long threads = a.total_kv * a.n_kv * (D / 8);
+            hipLaunchKernelGGL((relpos_dkv_join_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, s, a);
+            VDK_HIP(hipGetLastError());
+        }
     }
     if (a.d_dist) {
         hipLaunchKernelGGL(relpos_dbias_kernel, dim3(cdiv(2 * a.radius + 1, 64), a.n_heads), dim3(1024), 0, s, a);
@@ -524,7 +585,9 @@ extern "C" size_t vdk_relpos_attention_backward_workspace_size(const vdk_attn_pl
     if (guarded([&] {
             require(p, "relpos_attention_backward: NULL plan");
             require(bias_radius >= 0 && bias_radius <= 4096, "relpos_attention_backward: bias_radius must be 0 .. 4096");
-            n = up16((size_t)p->n_heads * p->total_q * 4) + up16((size_t)p->n_heads * p->n_b32 * 4) +
+            const int parts = head_parts_of(p);
+            n = parts > 1 ? (size_t)parts * 2 * p->total_kv * p->n_kv * p->dim * 4 : 0;
+            n += up16((size_t)p->n_heads * p->total_q * 4) + up16((size_t)p->n_heads * p->n_b32 * 4) +
                 up16((size_t)p->n_b32 * sizeof(int2)) +
                 (bias_radius ? (size_t)p->n_heads * p->n_b32 * (2 * bias_radius + 1) * 4 : 0);
         }) != 0)
@@ -570,6 +633,9 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
         w += up16((size_t)p->n_heads * p->n_b32 * 4);
         f.span = reinterpret_cast<int2*>(w);
         w += up16((size_t)p->n_b32 * sizeof(int2));
+        f.head_parts = head_parts_of(p);
+        f.kv_part = reinterpret_cast<float*>(w);
+        if (f.head_parts > 1) w += (size_t)f.head_parts * 2 * p->total_kv * p->n_kv * p->dim * 4;
         f.part = reinterpret_cast<float*>(w);
         f.d_dist = g->d_dist_bias;
         f.clips = p->d_clips;
@@ -579,6 +645,7 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
         f.causal = p->causal;
         f.n_b32 = p->n_b32;
         f.total_q = p->total_q;
+        f.total_kv = p->total_kv;
         hipStream_t s = static_cast<hipStream_t>(stream);
         if (a->dtype == VDK_F16) p->dim == 64 ? launch_grad_t<half_t, 64>(p, f, a->cap > 0, s)
                                               : launch_grad_t<half_t, 128>(p, f, a->cap > 0, s);
