@@ -66,11 +66,33 @@ __device__ __forceinline__ float16v splat16(float x) {
     return v;
 }
 
-// The same registers less their rounded values v: what is still to be carried.
-template <class T>
-__device__ __forceinline__ void take8(float16v& s, typename Vec8<T>::type v, int c) {
+// x less the rounded value v[e] of a pair, exactly, in one instruction (a dot product with (-1, 0) or (0, -1)).
+__device__ __forceinline__ float less(float x, Vec8<half_t>::pair v, int e) {
+    using P = Vec8<half_t>::pair;
+    return e ? __builtin_amdgcn_fdot2(v, P{(half_t)0.0f, (half_t)-1.0f}, x, false)
+             : __builtin_amdgcn_fdot2(v, P{(half_t)-1.0f, (half_t)0.0f}, x, false);
+}
+__device__ __forceinline__ float less(float x, Vec8<bf16_t>::pair v, int e) {
+    uint32_t m = e ? 0xbf800000u : 0x0000bf80u;   // -1 in one half
+    asm("" : "+s"(m));   // (from a register: as an inline constant the instruction would take it for something else)
+    return __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(Vec8<bf16_t>::pair, m), x, false);
+}
+
+// Eight values in N 16-bit parts, each what the ones before have rounded away.
+template <class T, int N>
+__device__ __forceinline__ void split8(float16v x, typename Vec8<T>::type (&parts)[N]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[8 * c + j] -= (float)v[j];
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const auto p = pack2<T>(x[j], x[j + 1]);
+            parts[i][j] = p[0];
+            parts[i][j + 1] = p[1];
+            if (i + 1 < N) {
+                x[j] = less(x[j], p, 0);
+                x[j + 1] = less(x[j + 1], p, 1);
+            }
+        }
 }
 
 // The largest of three (no operand is a signalling NaN, which fmaxf would see to).
@@ -180,20 +202,32 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScoreMap {
     float mul, am, lim;   // q . k to y; w to s2; the |q . k| where |y| = 1/2
+    float c[5];           // s2 = x (c0 + c1 x^2 + .. + c4 x^8) of x = q . k below lim
 };
 
+constexpr double kTanh[5] = {1.0, -0.33333072, 0.13324828, -0.05298924, 0.01714132};
+
 inline ScoreMap score_map(float scale, float cap) {
-    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f};
-    return {scale / cap, cap * kLog2e, 0.5f * cap / scale};
+    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f, {}};
+    ScoreMap m{scale / cap, cap * kLog2e, 0.5f * cap / scale, {}};
+    const double y = (double)scale / cap;
+    double f = (double)cap * kLog2e * y;
+    for (int i = 0; i < 5; ++i, f *= y * y) m.c[i] = (float)(f * kTanh[i]);
+    return m;
+}
+
+// The factor of x in s2 below lim.
+__device__ __forceinline__ float score_poly(float x, const ScoreMap& m) {
+    const float z = x * x;
+    return __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, m.c[4], m.c[3]), m.c[2]), m.c[1]), m.c[0]);
 }
 
 __device__ __forceinline__ float tanh_small(float y) {
     const float z = y * y;
-    return y * __builtin_fmaf(
-                   z,
-                   __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 0.01714132f, -0.05298924f), 0.13324828f),
-                                  -0.33333072f),
-                   1.0f);
+    float p = (float)kTanh[4];
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = __builtin_fmaf(z, p, (float)kTanh[i]);
+    return y * p;
 }
 
 __device__ __forceinline__ float tanh_any(float y) {

@@ -103,35 +103,55 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(Fw
             float16v s = splat16(0.0f);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tk, kt, kk), qf[kk], s);
-            score_w<CAP>(s, a.map);
-            // s[r]: key k0 + 8 (r / 4) + 4 hl + r % 4 of query qi
+            // s[r]: key k0 + 8 (r / 4) + 4 hl + r % 4 of query qi.  s2 = mul * s + add, or with a cap's polynomial in
+            // mul's place; blocks that need more (large scores, masks, biases by element) are taken to s2 here
+            const int d0 = k0 - (qw + past);   // distances of the block: d0 - 31 .. d0 + 31
+            const bool near = R != 0 && d0 + 31 > -R && d0 - 31 < R;
+            float mul = am, add = d0 < 0 ? far_l : far_r;
+            bool poly = CAP;
+            if constexpr (CAP) {
+                float top = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) top = max3_abs(s[r], s[r + 1], top);
+                if (__any(top > a.map.lim)) {
+                    keep_branch();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = am * tanh_any(s[r] * a.map.mul);
+                    poly = false;
+                    mul = 1.0f;
+                }
+            }
+            auto to_s2 = [&](auto base) {
+                if (CAP && poly) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], score_poly(s[r], a.map), base(r));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, base(r));
+                }
+                poly = false;
+                mul = 1.0f;
+                add = 0.0f;
+            };
+            if (near) {
+                const float* t = tab + (d0 - lr + 4 * hl + R + kTabPad);
+                to_s2([&](int r) { return t[8 * (r >> 2) + (r & 3)]; });
+            } else if (add < -1e37f || (CAP && k0 + 32 > kfull)) {
+                // (a far bias of the lowest value takes the products in, as the near ones do)
+                keep_branch();
+                to_s2([&](int) { return add; });
+            }
             if (k0 + 32 > kfull) {
                 keep_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (k0 + 8 * (r >> 2) + 4 * hl + (r & 3) >= lim) s[r] = -INFINITY;
             }
-            const int d0 = k0 - (qw + past);   // distances of the block: d0 - 31 .. d0 + 31
-            const bool near = R != 0 && d0 + 31 > -R && d0 - 31 < R;
-            float mul = am, add = d0 < 0 ? far_l : far_r;
-            if (near) {
-                const float* t = tab + (d0 - lr + 4 * hl + R + kTabPad);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], am, t[8 * (r >> 2) + (r & 3)]);
-                mul = 1.0f;
-                add = 0.0f;
-            } else if (add < -1e37f) {   // a far bias of the lowest value takes the products in, as the near ones do
-                keep_branch();
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], am, add);
-                mul = 1.0f;
-                add = 0.0f;
-            }
             // p = exp2(s2 - m) and its sum; only where a lane's sum passes 2^13 (as in the first block) does the row's
             // maximum move, and p is taken again: no maximum is looked for in the others
             constexpr int kParts = !SPLIT ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
             V8 pb[2][kParts];
-            auto exponentials = [&] {
+            auto exponentials = [&](auto with_poly) {
                 float sum[2] = {0.0f, 0.0f};
                 const float minus = add - m;
 #pragma unroll
@@ -139,20 +159,21 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(Fw
                     float16v p;   // (eight of them, as pack8 takes them)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * cc + j], mul, minus));
+                        const float x = s[8 * cc + j];
+                        const float f = decltype(with_poly)::value ? score_poly(x, a.map) : mul;
+                        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, minus));
                         sum[j & 1] += p[j];
                     }
-#pragma unroll
-                    for (int i = 0; i < kParts; ++i) {
-                        pb[cc][i] = pack8<T>(p, 0);
-                        if (i + 1 < kParts) take8<T>(p, pb[cc][i], 0);
-                    }
+                    split8<T>(p, pb[cc]);
                 }
                 return sum[0] + sum[1];
             };
-            float sum = exponentials();
+            using No = std::integral_constant<bool, false>;
+            using Poly = std::integral_constant<bool, CAP>;
+            float sum = CAP && poly ? exponentials(Poly{}) : exponentials(No{});
             if (__any(!(sum < 8192.0f))) {
                 keep_branch();
+                if (CAP && poly) to_s2([&](int) { return add; });
                 float mx = __builtin_fmaf(max16(s), mul, add);
                 mx = fmaxf(mx, other_half(mx));
                 const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
@@ -162,7 +183,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(Fw
                 for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-                sum = exponentials();
+                sum = exponentials(No{});
             }
             l += sum;
 #pragma unroll
