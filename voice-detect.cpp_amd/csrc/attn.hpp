@@ -272,10 +272,12 @@ constexpr int kKeys = 64;     // rows of a step's tiles
 constexpr int kTabPad = 96;   // a tile of 64 x 32 that touches a distance inside (-R, R) reaches 95 past it
 
 // ---- packed layouts ----
-struct AttnClip {
-    long long q0, k0;   // first query and key
+// A work item: its clip, whole (one load instead of two in a row), and its first row.
+struct AttnTile {
+    long long q0, k0;       // the clip's first query and key
     int nq, nk, prefix;
     int b32;                // blocks of 32 queries before the clip's
+    int row, pad;
 };
 
 // Argument checks shared by the forward and the backward call.
@@ -284,13 +286,12 @@ void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a);
 
 }  // namespace vdk
 
-// Work lists hold (clip, first row) of 128 queries or keys, heaviest first.
+// Work lists: 128 queries and 128 keys an item, heaviest first, and the blocks
+// of 32 queries in order.
 struct vdk_attn_plan {
     int n_clips, n_heads, n_kv, dim, causal;
     long long total_q, total_kv;
-    std::vector<vdk::AttnClip> clips;
-    int n_q128, n_k128, n_b32;   // (n_b32: blocks of 32 queries)
-    void* device;                  // one allocation for all tables
-    vdk::AttnClip* d_clips;
-    int2 *d_q128, *d_k128;
+    int n_q128, n_k128, n_b32;
+    void* device;                  // one allocation for all lists
+    vdk::AttnTile *d_q128, *d_k128, *d_b32;
 };

@@ -18,8 +18,7 @@ struct FwdArgs {
     void* o;
     long long o_tok, o_head;
     float *o32, *lse;
-    const AttnClip* clips;
-    const int2* tiles;
+    const AttnTile* tiles;
     int n_tiles, n_heads, group, causal;
     long long total_q;
 };
@@ -36,23 +35,22 @@ struct FwdArgs {
 // dO) from o, and a bias's gradient sums dS over whole rows, where its terms
 // cancel and delta's error does not.
 template <class T, int D, int NW, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fwd_kernel(FwdArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int kTile = kKeys * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
     const int id = xcd_swizzle(blockIdx.x, gridDim.x);
     const int h = id / a.n_tiles;
-    const int2 tile = a.tiles[id - h * a.n_tiles];
-    const AttnClip c = a.clips[tile.x];
+    const AttnTile c = a.tiles[id - h * a.n_tiles];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, qw = tile.y + 32 * wave, qi = qw + lr;
+    const int past = c.nk - c.nq, qw = c.row + 32 * wave, qi = qw + lr;
     const int qr = qi < c.nq ? qi : c.nq - 1;
 
     // keys: [0, kend) for the workgroup, [0, kend_w) for the wave, [0, lim) for the lane's query
     auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
-    const int kend = max(last(min(tile.y + 32 * NW, c.nq) - 1), 0);
+    const int kend = max(last(min(c.row + 32 * NW, c.nq) - 1), 0);
     const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
     const int kfull = qw < c.nq ? last(qw) : 0;      // all 32 rows see the keys below
     const int lim = last(qr);
@@ -100,9 +98,16 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(Fw
         for (int kt = 0; kt < 2; ++kt) {
             const int k0 = kb + 32 * kt;
             if (kt && k0 >= kend_w) break;
+            V8 kf[D / 16], vf[D / 32];
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) kf[kk] = at.row_block(tk, kt, kk);
             float16v s = splat16(0.0f);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tk, kt, kk), qf[kk], s);
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(kf[kk], qf[kk], s);
+            // the first values' loads run beside the exponentials
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) vf[dt] = at.col_block(tv, 2 * kt, dt);
+            __builtin_amdgcn_sched_barrier(0);
             // s[r]: key k0 + 8 (r / 4) + 4 hl + r % 4 of query qi.  s2 = mul * s + add, or with a cap's polynomial in
             // mul's place; blocks that need more (large scores, masks, biases by element) are taken to s2 here
             const int d0 = k0 - (qw + past);   // distances of the block: d0 - 31 .. d0 + 31
@@ -190,9 +195,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void relpos_fwd_kernel(Fw
             for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                 for (int dt = 0; dt < D / 32; ++dt) {
-                    const V8 vt = at.col_block(tv, 2 * kt + cc, dt);
 #pragma unroll
-                    for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vt, pb[cc][i], o[dt]);
+                    for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vf[dt], pb[cc][i], o[dt]);
+                    if (cc == 0) vf[dt] = at.col_block(tv, 2 * kt + 1, dt);
                 }
         }
     };
@@ -371,7 +376,8 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         p.n_kv = n_kv_heads;
         p.dim = head_dim;
         p.causal = causal != 0;
-        std::vector<std::pair<long long, int2>> q128, k128;   // (work, tile)
+        std::vector<std::pair<long long, AttnTile>> q128, k128;   // (work, tile)
+        std::vector<AttnTile> lists;
         int b32 = 0;
         for (int c = 0; c < n_clips; ++c) {
             const long long nq = q_offsets[c + 1] - q_offsets[c], nk = kv_offsets[c + 1] - kv_offsets[c];
@@ -379,23 +385,27 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
             require(nq <= (1 << 30) && nk <= (1 << 30), "attn_plan: a clip may hold 2^30 frames at most");
             const long long pre = prefix ? prefix[c] : 0;
             require(pre >= 0 && pre <= nk, "attn_plan: a prefix must be 0 .. the clip's keys");
-            p.clips.push_back({q_offsets[c], kv_offsets[c], (int)nq, (int)nk, (int)pre, b32});
+            AttnTile t{q_offsets[c], kv_offsets[c], (int)nq, (int)nk, (int)pre, b32, 0, 0};
+            auto at = [&](long long row) {
+                t.row = (int)row;
+                return t;
+            };
             const long long past = nk - nq;
             auto seen = [&](long long q) { return p.causal ? std::max(0ll, std::min(nk, std::max(pre, past + q + 1))) : nk; };
             for (long long q = 0; q < nq; q += 128)
-                q128.push_back({seen(std::min(q + 128, nq) - 1), int2{c, (int)q}});
+                q128.push_back({seen(std::min(q + 128, nq) - 1), at(q)});
+            for (long long q = 0; q < nq; q += 32) lists.push_back(at(q));
             b32 += cdiv(nq, 32);
             require((long long)b32 * n_heads < (1 << 30) && k128.size() * n_heads < (1u << 30),
                     "attn_plan: too many tiles for one launch");
             for (long long k = 0; k < nk; k += 128) {
                 const long long first = p.causal && k >= pre ? std::max(0ll, k - past) : 0;   // the first query that sees it
-                k128.push_back({std::max(0ll, nq - first), int2{c, (int)k}});
+                k128.push_back({std::max(0ll, nq - first), at(k)});
             }
         }
         p.total_q = n_clips ? q_offsets[n_clips] : 0;
         p.total_kv = n_clips ? kv_offsets[n_clips] : 0;
         require(p.total_q <= (1ll << 36) && p.total_kv <= (1ll << 36), "attn_plan: too many frames");
-        std::vector<int2> lists;
         for (auto* l : {&q128, &k128}) {
             std::stable_sort(l->begin(), l->end(), [](const auto& x, const auto& y) { return x.first > y.first; });
             for (const auto& t : *l) lists.push_back(t.second);
@@ -403,15 +413,14 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         p.n_q128 = (int)q128.size();
         p.n_k128 = (int)k128.size();
         p.n_b32 = b32;
-        const size_t nc = p.clips.size() * sizeof(AttnClip), nl = lists.size() * sizeof(int2);
-        if (vdk_device_count() > 0 && nc + nl > 0) {
-            VDK_HIP(hipMalloc(&p.device, nc + nl));
-            p.d_clips = static_cast<AttnClip*>(p.device);
-            p.d_q128 = reinterpret_cast<int2*>(static_cast<char*>(p.device) + nc);
+        const size_t bytes = lists.size() * sizeof(AttnTile);
+        if (vdk_device_count() > 0 && bytes > 0) {
+            VDK_HIP(hipMalloc(&p.device, bytes));
+            p.d_b32 = static_cast<AttnTile*>(p.device);
+            p.d_q128 = p.d_b32 + p.n_b32;
             p.d_k128 = p.d_q128 + p.n_q128;
             try {
-                VDK_HIP(hipMemcpy(p.d_clips, p.clips.data(), nc, hipMemcpyHostToDevice));
-                VDK_HIP(hipMemcpy(p.d_q128, lists.data(), nl, hipMemcpyHostToDevice));
+                VDK_HIP(hipMemcpy(p.device, lists.data(), bytes, hipMemcpyHostToDevice));
                 *plan = new vdk_attn_plan(p);
             } catch (...) {
                 (void)hipFree(p.device);
@@ -435,7 +444,7 @@ extern "C" int vdk_relpos_attention(const vdk_attn_plan* p, const vdk_relpos_att
         if (p->total_q == 0) return;
         FwdArgs f{a->q, a->k, a->v, a->q_tok, a->q_head, a->k_tok, a->k_head, a->v_tok, a->v_head, a->dist_bias,
                   a->dist_bias ? a->bias_radius : 0, score_map(a->scale, a->cap), a->o, a->o_tok, a->o_head, a->o_f32,
-                  a->lse, p->d_clips, nullptr, 0, p->n_heads, p->n_heads / p->n_kv, p->causal, p->total_q};
+                  a->lse, nullptr, 0, p->n_heads, p->n_heads / p->n_kv, p->causal, p->total_q};
         hipStream_t s = static_cast<hipStream_t>(stream);
         if (a->dtype == VDK_F16)
             p->dim == 64 ? launch_fwd_t<half_t, 64>(p, f, a->cap > 0, s) : launch_fwd_t<half_t, 128>(p, f, a->cap > 0, s);

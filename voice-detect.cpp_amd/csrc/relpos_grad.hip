@@ -3,9 +3,9 @@
 // With P = exp(s - lse), delta_i = sum_d o_i dO_i (o unrounded), dP = dO V^T:
 //   dV = P^T dO, dS = P (dP - delta), d bias by distance = diagonal sums of dS,
 //   dx = dS (1 - tanh^2) with a cap, dQ = scale dx K, dK = scale dx^T Q.
-// Two kernels, each recomputing P from lse, so that no sum needs atomics: one
-// owns 128 queries (delta, dQ, the bias), one 128 keys (dK, dV; the heads that
-// share them in turn).  Seven products where one kernel with atomics has five.
+// Two kinds of tiles, each recomputing P from lse, so that no sum needs atomics:
+// 128 queries (dQ, the bias) or 128 keys (dK, dV; the heads that share them in
+// turn).  Seven products where one kernel with atomics has five.
 //
 // P is carried times 2^8 and, in f16, dx times a power of two that brings the
 // row's (block's) largest |dO| to 2^-4 .. 2^-3: both are rounded to 16 bits as
@@ -28,9 +28,8 @@ struct GradArgs {
     long long dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
     float *delta, *most, *part, *d_dist;   // [heads][total_q], [heads][blocks], [heads][blocks][2 R + 1], the result
     int2* span;                            // [blocks]: the distances a block of 32 queries has written
-    const AttnClip* clips;
-    const int2* tiles;
-    int n_tiles, n_heads, n_kv, group, causal, n_b32;
+    const AttnTile *q_tiles, *k_tiles, *blocks;
+    int n_q, n_k, n_heads, n_kv, group, causal, n_b32;
     long long total_q, total_kv;
     float* kv_part;                        // [head_parts][2][total_kv][n_kv][D], where the heads of a key head are split
     int head_parts;
@@ -69,23 +68,63 @@ __device__ __forceinline__ void add_diagonals(const float16v& ds, float (&acc)[5
     }
 }
 
+// delta and the largest |dO| of 32 queries of a head, eight lanes a row.
+template <class T, int D>
+__global__ __launch_bounds__(256) void relpos_delta_kernel(GradArgs a) {
+    __shared__ float top[32];
+    const int h = blockIdx.y, row = threadIdx.x >> 3, part = threadIdx.x & 7;
+    const AttnTile c = a.blocks[blockIdx.x];
+    const int qi = c.row + row;
+    float delta = 0.0f, most = 0.0f;
+    if (qi < c.nq) {
+        const T* dp = static_cast<const T*>(a.d_o) + (c.q0 + qi) * a.do_tok + (long long)h * a.do_head;
+        const float* op = a.o32 + ((c.q0 + qi) * a.n_heads + h) * D;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            const int at = 64 * j + 8 * part;
+            const auto d = *reinterpret_cast<const typename Vec8<T>::type*>(dp + at);
+            const float4v o0 = *reinterpret_cast<const float4v*>(op + at), o1 = *reinterpret_cast<const float4v*>(op + at + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                delta = __builtin_fmaf((float)d[e], e < 4 ? o0[e & 3] : o1[e & 3], delta);
+                most = fmaxf(most, fabsf((float)d[e]));
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) {
+        delta += __shfl_xor(delta, off, 64);
+        most = fmaxf(most, __shfl_xor(most, off, 64));
+    }
+    if (part == 0) {
+        if (qi < c.nq) a.delta[h * a.total_q + c.q0 + qi] = delta;
+        top[row] = most;
+    }
+    if constexpr (kScaled<T>) {
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            most = top[threadIdx.x];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 32));
+            if (threadIdx.x == 0) a.most[(long long)h * a.n_b32 + blockIdx.x] = most;
+        }
+    }
+}
+
 // dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
+__device__ __forceinline__ void dq_tile(const GradArgs& a, int id, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
-    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-    const int h = id / a.n_tiles;
-    const int2 tile = a.tiles[id - h * a.n_tiles];
-    const AttnClip c = a.clips[tile.x];
+    const int h = id / a.n_q;
+    const AttnTile c = a.q_tiles[id - h * a.n_q];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, qw = tile.y + 32 * wave, qi = qw + lr;
+    const int past = c.nk - c.nq, qw = c.row + 32 * wave, qi = qw + lr;
     const int qr = qi < c.nq ? qi : c.nq - 1;
     auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
-    const int kend = max(last(min(tile.y + 32 * NW, c.nq) - 1), 0);
+    const int kend = max(last(min(c.row + 32 * NW, c.nq) - 1), 0);
     const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
     const int kfull = qw < c.nq ? last(qw) : 0;
     const int lim = last(qr);
@@ -102,36 +141,25 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
     };
     if (kend > 0) fetch(0, 0);
 
-    // the row's q, dO, delta and largest |dO|
+    // the row's q, dO and largest |dO|
     const T* qp = static_cast<const T*>(a.q) + (c.q0 + qr) * a.q_tok + (long long)h * a.q_head;
     const T* dp = static_cast<const T*>(a.d_o) + (c.q0 + qr) * a.do_tok + (long long)h * a.do_head;
-    const float* op = a.o32 + ((c.q0 + qr) * a.n_heads + h) * D;
     V8 qf[D / 16], df[D / 16];
-    float delta = 0.0f, most = 0.0f;
+    float most = 0.0f;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
         qf[kk] = *reinterpret_cast<const V8*>(qp + 16 * kk + 8 * hl);
         df[kk] = *reinterpret_cast<const V8*>(dp + 16 * kk + 8 * hl);
-        const float4v o0 = *reinterpret_cast<const float4v*>(op + 16 * kk + 8 * hl),
-                      o1 = *reinterpret_cast<const float4v*>(op + 16 * kk + 8 * hl + 4);
+        if constexpr (kScaled<T>) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = (float)df[kk][e];
-            delta = __builtin_fmaf(d, e < 4 ? o0[e & 3] : o1[e & 3], delta);
-            most = fmaxf(most, fabsf(d));
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)df[kk][e]));
         }
     }
-    delta += other_half(delta);
-    most = fmaxf(most, other_half(most));
+    if constexpr (kScaled<T>) most = fmaxf(most, other_half(most));
+    const float delta = a.delta[h * a.total_q + c.q0 + qr];
     const float lse = a.lse[h * a.total_q + c.q0 + qr];
     const float L2 = qi < c.nq && !(lse < -1e30f) ? lse * kLog2e - kPShift : FLT_MAX;
     const float sc = kScaled<T> ? scale_of(most) : 0x1p-8f, nd = -delta * sc;
-    if (qi < c.nq && hl == 0) a.delta[h * a.total_q + c.q0 + qi] = delta;
-    if (qw < c.nq) {
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-        if (lane == 0) a.most[h * a.n_b32 + c.b32 + (qw >> 5)] = most;
-    }
     const int R = BIAS ? a.radius : 0;
     float far_l = 0.0f, far_r = 0.0f;
     if constexpr (BIAS) {
@@ -283,23 +311,20 @@ __global__ __launch_bounds__(256, 2) void relpos_dq_kernel(GradArgs a) {
 // through LDS, the heads that share the keys one after the other, or a part of
 // them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
+__device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 and -delta sc of a step's queries
     float* tab = rows + 256;
-    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-    const int of = id / a.n_tiles, kvh = of / a.head_parts, hp = of - kvh * a.head_parts;
+    const int of = id / a.n_k, kvh = of / a.head_parts, hp = of - kvh * a.head_parts;
     const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
-    const int2 tile = a.tiles[id - of * a.n_tiles];
-    const AttnClip c = a.clips[tile.x];
+    const AttnTile c = a.k_tiles[id - of * a.n_k];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, kw = tile.y + 32 * wave, ki = kw + lr;
+    const int past = c.nk - c.nq, kw = c.row + 32 * wave, ki = kw + lr;
     const int kr = ki < c.nk ? ki : c.nk - 1;
     // the first query that sees a key of the tile, down to a whole step
-    const int q_first = a.causal && tile.y >= c.prefix ? max(tile.y - past, 0) & ~63 : 0;
+    const int q_first = a.causal && c.row >= c.prefix ? max(c.row - past, 0) & ~63 : 0;
     const int per_head = q_first < c.nq ? (c.nq - q_first + 63) >> 6 : 0, steps = per_head * heads;
 
     const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
@@ -478,7 +503,19 @@ __global__ __launch_bounds__(256, 2) void relpos_dkv_kernel(GradArgs a) {
         }
 }
 
-// The parts of relpos_dkv_kernel added up, 8 values a thread.
+// Both in one launch, the longer tiles of dK and dV first: the tiles of one fill the chip while the other's last ones run.
+template <class T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int b = blockIdx.x;
+    if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
+        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS>(a, xcd_swizzle(b, n_dkv), smem);
+    } else {
+        dq_tile<T, D, CAP, BIAS>(a, xcd_swizzle(b - n_dkv8, gridDim.x - n_dkv8), smem);
+    }
+}
+
+// The parts of dkv_tile added up, 8 values a thread.
 template <class T, int D>
 __global__ __launch_bounds__(256) void relpos_dkv_join_kernel(GradArgs a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / (D / 8);
@@ -536,26 +573,18 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 template <class T, int D, bool CAP, bool BIAS>
 void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
-    const int tab = BIAS ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0;
-    const int tiles = 4 * kKeys * D * 2;
-    if (p->n_q128) {
-        auto kern = relpos_dq_kernel<T, D, CAP, BIAS>;
-        const int lds = tiles + (BIAS ? tab + 16 + 4 * 512 * 4 : 0);
-        if (lds > 65536)
-            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        a.tiles = p->d_q128;
-        a.n_tiles = p->n_q128;
-        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(256), lds, s, a);
+    if (p->n_b32) {
+        hipLaunchKernelGGL((relpos_delta_kernel<T, D>), dim3(p->n_b32, a.n_heads), dim3(256), 0, s, a);
         VDK_HIP(hipGetLastError());
     }
-    if (p->n_k128) {
-        auto kern = relpos_dkv_kernel<T, D, CAP, BIAS>;
-        const int lds = tiles + 1024 + tab;
+    const long long n_dkv = (long long)a.n_k * a.n_kv * a.head_parts, n_dkv8 = (n_dkv + 7) / 8 * 8;
+    const long long n = n_dkv8 + (long long)a.n_q * a.n_heads;
+    if (n > 0) {
+        auto kern = relpos_grad_kernel<T, D, CAP, BIAS>;
+        const int lds = 4 * kKeys * D * 2 + 1024 + (BIAS ? 4 * (2 * a.radius + 1 + 2 * kTabPad) + 16 + 4 * 512 * 4 : 0);
         if (lds > 65536)
             VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        a.tiles = p->d_k128;
-        a.n_tiles = p->n_k128;
-        hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_kv * a.head_parts), dim3(256), lds, s, a);
+        hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), lds, s, a, (int)n_dkv, (int)n_dkv8);
         VDK_HIP(hipGetLastError());
         if (a.head_parts > 1) {
             const long long threads = a.total_kv * a.n_kv * (D / 8);
@@ -638,7 +667,11 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
         if (f.head_parts > 1) w += (size_t)f.head_parts * 2 * p->total_kv * p->n_kv * p->dim * 4;
         f.part = reinterpret_cast<float*>(w);
         f.d_dist = g->d_dist_bias;
-        f.clips = p->d_clips;
+        f.q_tiles = p->d_q128;
+        f.k_tiles = p->d_k128;
+        f.blocks = p->d_b32;
+        f.n_q = p->n_q128;
+        f.n_k = p->n_k128;
         f.n_heads = p->n_heads;
         f.n_kv = p->n_kv;
         f.group = p->n_heads / p->n_kv;
