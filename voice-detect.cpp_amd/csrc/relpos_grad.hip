@@ -314,7 +314,7 @@ template <class T, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
-    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 and -delta sc of a step's queries
+    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 (without a cap by am) and -delta of a step's queries
     float* tab = rows + 256;
     const int of = id / a.n_k, kvh = of / a.head_parts, hp = of - kvh * a.head_parts;
     const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
@@ -341,7 +341,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
     dmo.init(db_row, wave, lane);
     float row_v = 0.0f;   // this thread's entry of the next step's rows[]
     auto step_scale = [&](int h, int q) {   // from the step's largest |dO|
-        if constexpr (!kScaled<T>) return 0x1p-8f;
+        if constexpr (!kScaled<T>) return 1.0f;
         const float* p = a.most + h * a.n_b32 + c.b32 + (q >> 5);
         return scale_of(q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
     };
@@ -356,9 +356,9 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
             const long long at = h * a.total_q + c.q0 + min(qi, c.nq - 1);
             if (threadIdx.x < 64) {
                 const float lse = a.lse[at];
-                row_v = qi < c.nq && !(lse < -1e30f) ? kPShift - lse * kLog2e : -FLT_MAX;
+                row_v = qi < c.nq && !(lse < -1e30f) ? (kPShift - lse * kLog2e) * (CAP ? 1.0f : 1.0f / a.map.am) : -FLT_MAX;
             } else {
-                row_v = qi < c.nq ? -a.delta[at] * step_scale(h, q) : 0.0f;
+                row_v = qi < c.nq ? -a.delta[at] : 0.0f;
             }
         }
     };
@@ -371,7 +371,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
     const float am = a.map.am;
     TileReads<T, D> at;
     at.init(smem, lane);
-    float sc = 0x1p-8f, far_l = 0.0f, far_r = 0.0f;
+    float sc = 1.0f, far_l = 0.0f, far_r = 0.0f;
     if constexpr (kScaled<T>) {
         if (steps > 0) sc = step_scale(h0, q_first);
     }
@@ -409,34 +409,44 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
         for (int qt = 0; qt < 2; ++qt) {
             const int qs = q + 32 * qt;
             if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
-            float16v s = splat16(0.0f), p = splat16(0.0f);
+            // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki.  The sums start from the rows' own terms
+            float16v s, p;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4v l4 = *reinterpret_cast<const float4v*>(nl + 32 * qt + 8 * g + 4 * hl);
+                const float4v d4 = *reinterpret_cast<const float4v*>(nd + 32 * qt + 8 * g + 4 * hl);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * g + e] = CAP ? 0.0f : l4[e];
+                    p[4 * g + e] = d4[e];
+                }
+            }
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kf[kk], s);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(to, qt, kk), vf[kk], p);
             score_w<CAP>(s, a.map);
-            // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki
             const int d0 = kw - (qs + past);   // distances d0 - 31 .. d0 + 31
             const bool near = BIAS && d0 + 31 > -R && d0 - 31 < R;
-            float16v pr, ds;
+            float16v pr;
+            auto weights = [&](auto base) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4v l4 = *reinterpret_cast<const float4v*>(nl + 32 * qt + 8 * g + 4 * hl);
+                for (int g = 0; g < 4; ++g) {
+                    float4v l4 = {0, 0, 0, 0};
+                    if constexpr (CAP) l4 = *reinterpret_cast<const float4v*>(nl + 32 * qt + 8 * g + 4 * hl);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pr[4 * g + e] = l4[e];
-            }
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __builtin_fmaf(s[4 * g + e], am, base(4 * g + e));
+                        pr[4 * g + e] = __builtin_amdgcn_exp2f(CAP ? x + l4[e] : x);
+                    }
+                }
+            };
             if (near) {
                 const float* t = tab + (d0 + lr - 4 * hl + R + kTabPad);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, t[-(8 * (r >> 2) + (r & 3))]) + pr[r]);
-            } else if (BIAS) {
-                const float far = d0 < 0 ? far_l : far_r;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, far) + pr[r]);
+                weights([&](int r) { return t[-(8 * (r >> 2) + (r & 3))]; });
             } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, pr[r]));
+                const float far = d0 < 0 ? far_l : far_r;
+                weights([&](int) { return far; });
             }
             if (a.causal && kw + 31 >= max(c.prefix, past + qs + 1)) {
                 keep_branch();
@@ -444,13 +454,9 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
                 for (int r = 0; r < 16; ++r)
                     if (ki >= max(c.prefix, past + qs + 8 * (r >> 2) + 4 * hl + (r & 3) + 1)) pr[r] = 0.0f;
             }
+            float16v& ds = p;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4v d4 = *reinterpret_cast<const float4v*>(nd + 32 * qt + 8 * g + 4 * hl);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    ds[4 * g + e] = pr[4 * g + e] * __builtin_fmaf(p[4 * g + e], sc, d4[e]);
-            }
+            for (int r = 0; r < 16; ++r) ds[r] = pr[r] * (kScaled<T> ? p[r] * sc : p[r]);
             if constexpr (CAP) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] *= __builtin_fmaf(-s[r], s[r], 1.0f);
@@ -505,7 +511,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
 
 // Both in one launch, the longer tiles of dK and dV first: the tiles of one fill the chip while the other's last ones run.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int b = blockIdx.x;
     if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
