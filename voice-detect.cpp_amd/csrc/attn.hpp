@@ -130,26 +130,34 @@ __device__ __forceinline__ int tile_at(int row, int chunk) {   // byte offset
     return row * (2 * D) + ((chunk ^ tile_swz<D>(row)) << 4);
 }
 
+// dma16 with a wave-uniform offset besides the lane's (the range check covers
+// both).  Five wait states stand before it: the compiler, which does not see a
+// buffer instruction here, may bring a scalar operand back from a vector
+// register (a spill) right before, and that write takes as long to be seen.
+__device__ __forceinline__ void dma16_at(uint8_t* lds_dst, int4v rsrc, uint32_t voff, uint32_t soff) {
+    const uint32_t m0v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)lds_dst);
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff), "{m0}"(m0v)
+                 : "memory");
+}
+
 // ROWS rows from `src` (row stride in bytes, `valid` of them exist, the others
-// read as zero) into an LDS tile by DMA, spread over NW waves.
+// read as zero) into an LDS tile by DMA, spread over NW waves.  One instruction
+// of all waves takes a multiple of 16 rows, whose swizzles repeat: one lane
+// offset serves them all.
 template <int D, int ROWS, int NW>
 struct TileDma {
-    static constexpr int kOps = ROWS * D / 512;             // 1 KB each
-    static constexpr int kPer = (kOps + NW - 1) / NW;
-    uint32_t voff[kPer];
+    static constexpr int kRows = NW * 512 / D;              // rows of one instruction of all waves
+    static_assert(kRows % 16 == 0 && ROWS % kRows == 0, "whole instructions of whole swizzle periods");
+    uint32_t voff;
     __device__ __forceinline__ void init(uint32_t row_bytes, int wave, int lane) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int i = (j * NW + wave) * 64 + lane, row = i / (D / 8), pos = i % (D / 8);
-            voff[j] = row * row_bytes + ((pos ^ tile_swz<D>(row)) << 4);
-        }
+        const int i = wave * 64 + lane, row = i / (D / 8), pos = i % (D / 8);
+        voff = row * row_bytes + ((pos ^ tile_swz<D>(row)) << 4);
     }
     __device__ __forceinline__ void load(uint8_t* lds, const void* src, uint32_t row_bytes, int valid, int wave) const {
         const int n = valid < ROWS ? valid : ROWS;
         const int4v rsrc = dma_rsrc(src, n > 0 ? (uint32_t)(n - 1) * row_bytes + 2 * D : 0);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-            if (kOps % NW == 0 || j * NW + wave < kOps) dma16(lds + (j * NW + wave) * 1024, rsrc, voff[j]);
+        for (int j = 0; j < ROWS / kRows; ++j) dma16_at(lds + (j * NW + wave) * 1024, rsrc, voff, j * kRows * row_bytes);
     }
 };
 

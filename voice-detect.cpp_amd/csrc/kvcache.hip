@@ -272,13 +272,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(PagedArgs a)
             const int left = k1 - key, n = pg < 0 || left <= 0 ? 0 : left < 16 ? left : 16;
             const uint32_t bytes = n * kRow;
             const int4v rk = dma_rsrc(a.k + rows[t] * kRow, bytes), rv = dma_rsrc(a.v + rows[t] * kRow, bytes);
-            // five wait states between a vector write of a scalar (readfirstlane) and a buffer instruction that
-            // reads it, which the compiler does not count for instructions in inline assembly
-            asm volatile("s_nop 4" ::"s"(rk), "s"(rv));
 #pragma unroll
             for (int j = 0; j < 16 * kRow / 1024; ++j) {
-                dma16(dst + t * 16 * kRow + j * 1024, rk, voff[j]);
-                dma16(dst + S::kTile + t * 16 * kRow + j * 1024, rv, voff[j]);
+                dma16_at(dst + t * 16 * kRow + j * 1024, rk, voff[j], 0);
+                dma16_at(dst + S::kTile + t * 16 * kRow + j * 1024, rv, voff[j], 0);
             }
         }
         // lanes 0 .. 31: the keys' scales, 32 .. 63: the values' (past the part: some row of a page, not used)

@@ -423,6 +423,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
             }
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kf[kk], s);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(to, qt, kk), vf[kk], p);
             score_w<CAP>(s, a.map);
@@ -439,6 +440,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
                         const float x = __builtin_fmaf(s[4 * g + e], am, base(4 * g + e));
                         pr[4 * g + e] = __builtin_amdgcn_exp2f(CAP ? x + l4[e] : x);
                     }
+                    if (g & 1) __builtin_amdgcn_sched_barrier(0);   // (eight loads ahead, no more: registers)
                 }
             };
             if (near) {
