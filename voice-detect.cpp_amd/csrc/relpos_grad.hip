@@ -513,7 +513,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* sme
 
 // Both in one launch, the longer tiles of dK and dV first: the tiles of one fill the chip while the other's last ones run.
 template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int b = blockIdx.x;
     if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
