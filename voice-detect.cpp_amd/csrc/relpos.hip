@@ -34,10 +34,12 @@ struct FwdArgs {
 // or three of bf16, 22 or 24 bits of it.  The backward pass takes delta = sum(o
 // dO) from o, and a bias's gradient sums dS over whole rows, where its terms
 // cancel and delta's error does not.
-template <class T, int D, int NW, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fwd_kernel(FwdArgs a) {
+// NARROW (launches of few tiles): the four waves share 32 queries and take 32
+// keys each of a step's 128; their outputs are joined through LDS.
+template <class T, int D, bool CAP, bool SPLIT, bool NARROW>
+__global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void relpos_fwd_kernel(FwdArgs a) {
     using V8 = typename Vec8<T>::type;
-    constexpr int kTile = kKeys * D * 2;
+    constexpr int NW = 4, kRows = NARROW ? 32 : 128, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
     const int id = xcd_swizzle(blockIdx.x, gridDim.x);
@@ -45,12 +47,12 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fw
     const AttnTile c = a.tiles[id - h * a.n_tiles];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, qw = c.row + 32 * wave, qi = qw + lr;
+    const int past = c.nk - c.nq, qw = c.row + (NARROW ? 0 : 32 * wave), qi = qw + lr;
     const int qr = qi < c.nq ? qi : c.nq - 1;
 
     // keys: [0, kend) for the workgroup, [0, kend_w) for the wave, [0, lim) for the lane's query
     auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
-    const int kend = max(last(min(c.row + 32 * NW, c.nq) - 1), 0);
+    const int kend = max(last(min(c.row + kRows, c.nq) - 1), 0);
     const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
     const int kfull = qw < c.nq ? last(qw) : 0;      // all 32 rows see the keys below
     const int lim = last(qr);
@@ -58,7 +60,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fw
     const uint32_t kb_row = (uint32_t)a.k_tok * 2, vb_row = (uint32_t)a.v_tok * 2;
     const T* kp = static_cast<const T*>(a.k) + c.k0 * a.k_tok + (long long)(h / a.group) * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + c.k0 * a.v_tok + (long long)(h / a.group) * a.v_head;
-    TileDma<D, kKeys, NW> dk, dv;
+    TileDma<D, kStep, NW> dk, dv;
     dk.init(kb_row, wave, lane);
     dv.init(vb_row, wave, lane);
     auto fetch = [&](int kb, int buf) {
@@ -85,19 +87,18 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fw
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) o[dt] = splat16(0.0f);
     TileReads<T, D> at;
-    at.init(smem, lane);
+    at.init(smem + (NARROW ? wave * (64 * D) : 0), lane);
     float m = -FLT_MAX, l = 0.0f;
     const float am = a.map.am;
     auto step = [&](int kb, int buf) {
         wait_vmcnt<0>();
         lds_barrier();   // this tile is there, and the other buffer is no longer read
-        if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
-        if (kb >= kend_w) return;
+        if (kb + kStep < kend) fetch(kb + kStep, buf ^ 1);
         const int tk = buf * 2 * kTile, tv = tk + kTile;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const int k0 = kb + 32 * kt;
-            if (kt && k0 >= kend_w) break;
+        for (int kt = 0; kt < (NARROW ? 1 : 2); ++kt) {
+            const int k0 = kb + 32 * (NARROW ? wave : kt);
+            if (k0 >= kend_w) break;
             V8 kf[D / 16], vf[D / 32];
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) kf[kk] = at.row_block(tk, kt, kk);
@@ -201,31 +202,63 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 2 : CAP ? 3 : 4) void relpos_fw
                 }
         }
     };
-    for (int kb = 0; kb < kend; kb += 2 * kKeys) {
+    for (int kb = 0; kb < kend; kb += 2 * kStep) {
         step(kb, 0);
-        if (kb + kKeys < kend) step(kb + kKeys, 1);
+        if (kb + kStep < kend) step(kb + kStep, 1);
+    }
+    l += other_half(l);
+    float f[NW];
+    float* js = reinterpret_cast<float*>(smem);   // [wave][register][lane], then maxima and sums [wave][2][lane]
+    if constexpr (NARROW) {
+        float* ml = js + NW * (D / 2) * 64;
+        __syncthreads();   // the tiles are no longer read
+#pragma unroll
+        for (int r = 0; r < D / 2; ++r) js[(wave * (D / 2) + r) * 64 + lane] = o[r >> 4][r & 15];
+        ml[wave * 128 + lane] = m;
+        ml[wave * 128 + 64 + lane] = l;
+        __syncthreads();
+        m = -FLT_MAX;
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w * 128 + lane]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(ml[w * 128 + lane] - m);
+            l = __builtin_fmaf(f[w], ml[w * 128 + 64 + lane], l);
+        }
     }
     if (qi >= c.nq) return;
-    l += other_half(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* op = static_cast<T*>(a.o) + (c.q0 + qi) * a.o_tok + (long long)h * a.o_head;
     float* fp = a.o32 ? a.o32 + ((c.q0 + qi) * a.n_heads + h) * D : nullptr;
+    auto put = [&](int i, float4v v) {   // registers 4 i .. 4 i + 3
+        v *= float4v{inv, inv, inv, inv};
+        const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * hl;
+        uint2 u;
+        u.x = __builtin_bit_cast(uint32_t, pack2<T>(v[0], v[1]));
+        u.y = __builtin_bit_cast(uint32_t, pack2<T>(v[2], v[3]));
+        *reinterpret_cast<uint2*>(op + d) = u;
+        if (fp) *reinterpret_cast<float4v*>(fp + d) = v;
+    };
+    if constexpr (NARROW) {
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+        for (int j = 0; j < D / 32; ++j) {
+            const int i = wave * (D / 32) + j;
+            float4v v = {0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float4v v;
+            for (int w = 0; w < NW; ++w)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = o[dt][4 * g + e] * inv;
-            const auto lo = pack2<T>(v[0], v[1]), hi = pack2<T>(v[2], v[3]);
-            const int d = 32 * dt + 8 * g + 4 * hl;
-            uint2 u;
-            u.x = __builtin_bit_cast(uint32_t, lo);
-            u.y = __builtin_bit_cast(uint32_t, hi);
-            *reinterpret_cast<uint2*>(op + d) = u;
-            if (fp) *reinterpret_cast<float4v*>(fp + d) = v;
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(f[w], js[(w * (D / 2) + 4 * i + e) * 64 + lane], v[e]);
+            put(i, v);
         }
-    if (a.lse && hl == 0) {
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const float16v& x = o[i >> 2];
+            put(i, float4v{x[4 * (i & 3)], x[4 * (i & 3) + 1], x[4 * (i & 3) + 2], x[4 * (i & 3) + 3]});
+        }
+    }
+    if (a.lse && hl == 0 && (!NARROW || wave == 0)) {
         // (a row of the lowest value only: the value itself, its sum lies far below the last bit)
         const float v = m > -FLT_MAX ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -FLT_MAX;
         a.lse[h * a.total_q + c.q0 + qi] = l == 0.0f ? -INFINITY : v;
@@ -305,17 +338,24 @@ void check_buckets(const void* src, const void* dst, int n_buckets, int n_heads,
     require(R >= 1 && R <= kMaxRadius, w + ": bias_radius must be 1 .. 4096");
 }
 
-template <class T, int D, bool CAP, bool SPLIT>
-void launch_fwd(const vdk_attn_plan* p, FwdArgs a, hipStream_t s) {
-    constexpr int NW = 4;
-    const size_t lds = 4 * kKeys * D * 2 + (a.radius ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0);
-    auto kern = relpos_fwd_kernel<T, D, NW, CAP, SPLIT>;
+template <class T, int D, bool CAP, bool SPLIT, bool NARROW>
+void launch_tiles(const vdk_attn_plan* p, FwdArgs a, size_t lds, hipStream_t s) {
+    auto kern = relpos_fwd_kernel<T, D, CAP, SPLIT, NARROW>;
     if (lds > 65536)
         VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    a.tiles = p->d_q128;
-    a.n_tiles = p->n_q128;
-    hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(64 * NW), lds, s, a);
+    a.tiles = NARROW ? p->d_b32 : p->d_q128;
+    a.n_tiles = NARROW ? p->n_b32 : p->n_q128;
+    hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(256), lds, s, a);
     VDK_HIP(hipGetLastError());
+}
+
+template <class T, int D, bool CAP, bool SPLIT>
+void launch_fwd(const vdk_attn_plan* p, const FwdArgs& a, hipStream_t s) {
+    const size_t tab = a.radius ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0, wide = 4 * kKeys * D * 2 + tab;
+    const size_t narrow = 8 * kKeys * D * 2 + std::max<size_t>(tab, 2048);
+    // below one tile of 128 queries a CU the keys are split as well
+    if ((long long)p->n_q128 * p->n_heads < 256 && narrow <= 163840) launch_tiles<T, D, CAP, SPLIT, true>(p, a, narrow, s);
+    else launch_tiles<T, D, CAP, SPLIT, false>(p, a, wide, s);
 }
 
 template <class T, int D>
