@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(RowArgs a) {
 // O^T (dims x heads) += V^T P^T, V^T by transposing LDS loads; e4m3 codes
 // become 16-bit values exactly on their way from LDS.  The scale of a key
 // multiplies its score, that of a value its p.
-constexpr int kStep = 32, kWaves = 4;
+constexpr int kStep = 32;
 
 struct PagedArgs {
     const uint8_t *k, *v;
@@ -182,7 +182,7 @@ __device__ __forceinline__ int ring_chunk(int row, int c) {
     return RB == 64 ? c ^ ((row >> 2) & 3) : RB == 128 ? c ^ ((row >> 1) & 7) : c ^ (row & 15);
 }
 
-template <class T, int D, bool QUANT>
+template <class T, int D, bool QUANT, int kWaves>
 struct PagedShape {
     static constexpr int kRow = QUANT ? D : 2 * D;
     static constexpr int kTile = kStep * kRow;                       // keys (or values) of a step
@@ -194,9 +194,9 @@ struct PagedShape {
     static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
 };
 
-template <class T, int D, bool QUANT, bool CAP>
+template <class T, int D, bool QUANT, bool CAP, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(PagedArgs a) {
-    using S = PagedShape<T, D, QUANT>;
+    using S = PagedShape<T, D, QUANT, kWaves>;
     using V8 = typename Vec8<T>::type;
     using PT = std::conditional_t<QUANT, bf16_t, T>;   // p times a value's scale may leave the range of f16
     using P8 = typename Vec8<PT>::type;
@@ -574,14 +574,27 @@ void check_paged(const vdk_kv_cache* c, const vdk_paged_attn* a) {
     require(a->max_len <= (1 << 30), w + ": max_len must be 2^30 at most");
 }
 
-template <class T, int D, bool QUANT, bool CAP>
-void launch_paged(PagedArgs a, int n_seqs, hipStream_t s) {
-    auto kern = paged_attn_kernel<T, D, QUANT, CAP>;
-    const int lds = PagedShape<T, D, QUANT>::kLds + 4 * (a.chunk >> a.page_shift) + 4 * std::min(a.group, 16) * a.span;
+template <class T, int D, bool QUANT, bool CAP, int kWaves>
+void launch_parts(const PagedArgs& a, int n, hipStream_t s) {
+    auto kern = paged_attn_kernel<T, D, QUANT, CAP, kWaves>;
+    const int lds = PagedShape<T, D, QUANT, kWaves>::kLds + 4 * (a.chunk >> a.page_shift) + 4 * std::min(a.group, 16) * a.span;
     if (lds > 65536)
         VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(kern, dim3((unsigned)n_seqs * a.kv * a.head_parts * a.splits), dim3(64 * kWaves), lds, s, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * kWaves), lds, s, a);
     VDK_HIP(hipGetLastError());
+}
+
+template <class T, int D, bool QUANT, bool CAP>
+void launch_paged(const PagedArgs& a, int n_seqs, hipStream_t s) {
+    const long long n = (long long)n_seqs * a.kv * a.head_parts * a.splits;
+    // below one workgroup a CU eight waves each: a launch is then as long as one wave's steps
+    bool few = n < 256;
+    if constexpr (PagedShape<T, D, QUANT, 8>::kRing <= 139264) {
+        if (few) launch_parts<T, D, QUANT, CAP, 8>(a, (int)n, s);
+    } else {
+        few = false;
+    }
+    if (!few) launch_parts<T, D, QUANT, CAP, 4>(a, (int)n, s);
     if (a.splits > 1) {
         hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)n_seqs * a.n_heads), dim3(64), 0, s, a);
         VDK_HIP(hipGetLastError());

@@ -562,9 +562,18 @@ __global__ __launch_bounds__(1024) void relpos_dbias_kernel(GradArgs a) {
     double sum = 0.0;
     if (i <= 2 * R) {
         const bool edge = i == 0 || i == 2 * R;
-        for (int b = row; b < a.n_b32; b += 16) {
-            const int2 s = a.span[b];
-            if (edge || (i - R >= s.x && i - R <= s.y)) sum += a.part[((long long)h * a.n_b32 + b) * (2 * R + 1) + i];
+        const float* p = a.part + (long long)h * a.n_b32 * (2 * R + 1) + i;
+        for (int b0 = row; b0 < a.n_b32; b0 += 16 * 8) {   // eight loads at a time
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int b = min(b0 + 16 * j, a.n_b32 - 1);
+                const int2 s = a.span[b];
+                const bool ok = b0 + 16 * j < a.n_b32 && (edge || (i - R >= s.x && i - R <= s.y));
+                v[j] = ok ? p[(long long)b * (2 * R + 1)] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += v[j];
         }
     }
     red[row][threadIdx.x & 63] = sum;
