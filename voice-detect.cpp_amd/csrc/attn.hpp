@@ -203,44 +203,49 @@ struct TileReads {
 // ---- scores ----
 // Scores are kept in units of log 2: s2 = am * w + bias2, with w = q . k without
 // a cap, else w = tanh(y), y = scale q . k / cap.  tanh(y) / y is an even function:
-// for |y| <= 1/2 a polynomial in y^2 (Chebyshev fit, 2.7e-8 relative) keeps the
-// score's relative precision, where 1 - 2 / (1 + exp(2 y)) would lose all below
-// 6e-8 cap.  Blocks with a larger |y| take both and choose by element.
+// a polynomial in y^2 (Chebyshev fits: degree 2 for |y| <= 0.15, 4e-8 relative;
+// degree 4 for |y| <= 1/2, 2.7e-8) keeps the score's relative precision, where
+// 1 - 2 / (1 + exp(2 y)) would lose all below 6e-8 cap.  A block goes by its
+// largest |y|; beyond 1/2 both forms are taken and chosen from by element.
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScoreMap {
-    float mul, am, lim;   // q . k to y; w to s2; the |q . k| where |y| = 1/2
-    float c[5];           // s2 = x (c0 + c1 x^2 + .. + c4 x^8) of x = q . k below lim
+    float mul, am;          // q . k to y; w to s2
+    float lim[2];           // the |q . k| where |y| = 0.15 and 1/2
+    float c[3], d[5];       // s2 = x (c0 + c1 x^2 + ..) of x = q . k below the first, with d below the second
 };
 
-constexpr double kTanh[5] = {1.0, -0.33333072, 0.13324828, -0.05298924, 0.01714132};
+constexpr float kTanhC[3] = {1.0f, -0.33331817f, 0.13153109f};
+constexpr float kTanhD[5] = {1.0f, -0.33333072f, 0.13324828f, -0.05298924f, 0.01714132f};
 
 inline ScoreMap score_map(float scale, float cap) {
-    if (cap == 0.0f) return {1.0f, scale * kLog2e, 0.0f, {}};
-    ScoreMap m{scale / cap, cap * kLog2e, 0.5f * cap / scale, {}};
+    ScoreMap m{1.0f, scale * kLog2e, {}, {}, {}};
+    if (cap == 0.0f) return m;
     const double y = (double)scale / cap;
+    m.mul = (float)y;
+    m.am = cap * kLog2e;
+    m.lim[0] = (float)(0.15 / y);
+    m.lim[1] = (float)(0.5 / y);
     double f = (double)cap * kLog2e * y;
-    for (int i = 0; i < 5; ++i, f *= y * y) m.c[i] = (float)(f * kTanh[i]);
+    for (int i = 0; i < 5; ++i, f *= y * y) {
+        if (i < 3) m.c[i] = (float)(f * kTanhC[i]);
+        m.d[i] = (float)(f * kTanhD[i]);
+    }
     return m;
 }
 
-// The factor of x in s2 below lim.
-__device__ __forceinline__ float score_poly(float x, const ScoreMap& m) {
-    const float z = x * x;
-    return __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, m.c[4], m.c[3]), m.c[2]), m.c[1]), m.c[0]);
-}
-
-__device__ __forceinline__ float tanh_small(float y) {
-    const float z = y * y;
-    float p = (float)kTanh[4];
+// c0 + c1 z + ..
+template <int N>
+__device__ __forceinline__ float horner(float z, const float (&c)[N]) {
+    float p = c[N - 1];
 #pragma unroll
-    for (int i = 3; i >= 0; --i) p = __builtin_fmaf(z, p, (float)kTanh[i]);
-    return y * p;
+    for (int i = N - 2; i >= 0; --i) p = __builtin_fmaf(z, p, c[i]);
+    return p;
 }
 
 __device__ __forceinline__ float tanh_any(float y) {
     const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * y);
-    return fabsf(y) < 0.5f ? tanh_small(y) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+    return fabsf(y) < 0.5f ? y * horner(y * y, kTanhD) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 // The largest of |a|, |b| and c.
@@ -258,13 +263,18 @@ __device__ __forceinline__ void score_w(V& s, const ScoreMap& m) {
         float top = 0.0f;
 #pragma unroll
         for (int r = 0; r < N; r += 2) top = max3_abs(s[r], s[r + 1], top);
-        if (__any(top > m.lim)) {
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int r = 0; r < N; ++r) s[r] = f(s[r] * m.mul);
+        };
+        if (!__any(top > m.lim[0])) {
+            each([](float y) { return y * horner(y * y, kTanhC); });
+        } else if (!__any(top > m.lim[1])) {
             keep_branch();
-#pragma unroll
-            for (int r = 0; r < N; ++r) s[r] = tanh_any(s[r] * m.mul);
+            each([](float y) { return y * horner(y * y, kTanhD); });
         } else {
-#pragma unroll
-            for (int r = 0; r < N; ++r) s[r] = tanh_small(s[r] * m.mul);
+            keep_branch();
+            each([](float y) { return tanh_any(y); });
         }
     }
 }
@@ -274,6 +284,18 @@ __device__ __forceinline__ void score_w(V& s, const ScoreMap& m) {
 __device__ __forceinline__ float bias2_of(float b) {
     const float x = b * kLog2e;
     return fabsf(b) == INFINITY ? b : fminf(fmaxf(x, -FLT_MAX), FLT_MAX);
+}
+
+// A workgroup's (head, tile) of `tiles` sorted heaviest first: every XCD serves
+// whole heads, whose keys and values its L2 then holds, and where they divide
+// evenly takes its heads' heavy tiles before any light one.
+__device__ __forceinline__ int2 head_tile(int bid, int tiles, int heads) {
+    if ((heads & 7) == 0) {
+        const int per = heads >> 3, j = bid >> 3, t = j / per;
+        return int2{(bid & 7) * per + j - t * per, t};
+    }
+    const int id = xcd_swizzle(bid, tiles * heads), h = id / tiles;
+    return int2{h, id - h * tiles};
 }
 
 constexpr int kKeys = 64;     // rows of a step's tiles

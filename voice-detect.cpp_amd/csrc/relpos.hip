@@ -42,9 +42,9 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
     constexpr int NW = 4, kRows = NARROW ? 32 : 128, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
-    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-    const int h = id / a.n_tiles;
-    const AttnTile c = a.tiles[id - h * a.n_tiles];
+    const int2 ht = head_tile(blockIdx.x, a.n_tiles, a.n_heads);
+    const int h = ht.x;
+    const AttnTile c = a.tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
     const int past = c.nk - c.nq, qw = c.row + (NARROW ? 0 : 32 * wave), qi = qw + lr;
@@ -114,28 +114,35 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
             const int d0 = k0 - (qw + past);   // distances of the block: d0 - 31 .. d0 + 31
             const bool near = R != 0 && d0 + 31 > -R && d0 - 31 < R;
             float mul = am, add = d0 < 0 ? far_l : far_r;
-            bool poly = CAP;
+            int poly = CAP ? 1 : 0;   // 1: the short polynomial, 2: the long one, 0: mul
             if constexpr (CAP) {
                 float top = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) top = max3_abs(s[r], s[r + 1], top);
-                if (__any(top > a.map.lim)) {
+                if (__any(top > a.map.lim[0])) {
                     keep_branch();
+                    poly = 2;
+                    if (__any(top > a.map.lim[1])) {
+                        keep_branch();
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = am * tanh_any(s[r] * a.map.mul);
-                    poly = false;
-                    mul = 1.0f;
+                        for (int r = 0; r < 16; ++r) s[r] = am * tanh_any(s[r] * a.map.mul);
+                        poly = 0;
+                        mul = 1.0f;
+                    }
                 }
             }
             auto to_s2 = [&](auto base) {
-                if (CAP && poly) {
+                if (CAP && poly == 1) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], score_poly(s[r], a.map), base(r));
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], horner(s[r] * s[r], a.map.c), base(r));
+                } else if (CAP && poly == 2) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], horner(s[r] * s[r], a.map.d), base(r));
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, base(r));
                 }
-                poly = false;
+                poly = 0;
                 mul = 1.0f;
                 add = 0.0f;
             };
@@ -166,7 +173,8 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float x = s[8 * cc + j];
-                        const float f = decltype(with_poly)::value ? score_poly(x, a.map) : mul;
+                        constexpr int kPoly = decltype(with_poly)::value;
+                        const float f = kPoly ? horner(x * x, a.map.c) : mul;
                         p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, minus));
                         sum[j & 1] += p[j];
                     }
@@ -174,9 +182,10 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
                 }
                 return sum[0] + sum[1];
             };
-            using No = std::integral_constant<bool, false>;
-            using Poly = std::integral_constant<bool, CAP>;
-            float sum = CAP && poly ? exponentials(Poly{}) : exponentials(No{});
+            using No = std::integral_constant<int, 0>;
+            using Short = std::integral_constant<int, CAP ? 1 : 0>;
+            if (CAP && poly == 2) to_s2([&](int) { return add; });
+            float sum = CAP && poly ? exponentials(Short{}) : exponentials(No{});
             if (__any(!(sum < 8192.0f))) {
                 keep_branch();
                 if (CAP && poly) to_s2([&](int) { return add; });

@@ -113,12 +113,13 @@ __global__ __launch_bounds__(256) void relpos_delta_kernel(GradArgs a) {
 
 // dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32.
 template <class T, int D, bool CAP, bool BIAS>
-__device__ __forceinline__ void dq_tile(const GradArgs& a, int id, uint8_t* smem) {
+__device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
-    const int h = id / a.n_q;
-    const AttnTile c = a.q_tiles[id - h * a.n_q];
+    const int2 ht = head_tile(bid, a.n_q, a.n_heads);
+    const int h = ht.x;
+    const AttnTile c = a.q_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
     const int past = c.nk - c.nq, qw = c.row + 32 * wave, qi = qw + lr;
@@ -311,14 +312,15 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int id, uint8_t* smem
 // through LDS, the heads that share the keys one after the other, or a part of
 // them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
 template <class T, int D, bool CAP, bool BIAS>
-__device__ __forceinline__ void dkv_tile(const GradArgs& a, int id, uint8_t* smem) {
+__device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kTile = kKeys * D * 2;
     float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 (without a cap by am) and -delta of a step's queries
     float* tab = rows + 256;
-    const int of = id / a.n_k, kvh = of / a.head_parts, hp = of - kvh * a.head_parts;
+    const int2 ht = head_tile(bid, a.n_k, a.n_kv * a.head_parts);
+    const int kvh = ht.x / a.head_parts, hp = ht.x - kvh * a.head_parts;
     const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
-    const AttnTile c = a.k_tiles[id - of * a.n_k];
+    const AttnTile c = a.k_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
     const int past = c.nk - c.nq, kw = c.row + 32 * wave, ki = kw + lr;
@@ -517,9 +519,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void relpos_grad_kernel(GradA
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int b = blockIdx.x;
     if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
-        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS>(a, xcd_swizzle(b, n_dkv), smem);
+        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS>(a, b, smem);
     } else {
-        dq_tile<T, D, CAP, BIAS>(a, xcd_swizzle(b - n_dkv8, gridDim.x - n_dkv8), smem);
+        dq_tile<T, D, CAP, BIAS>(a, b - n_dkv8, smem);
     }
 }
 
