@@ -121,6 +121,16 @@ FORWARD = [
 ]
 
 
+# layouts of many tiles (the wide kernel; those above are few enough for the one that splits the keys)
+WIDE = [
+    dict(nq=[130, 257, 64, 1], H=64, kv=16, D=64, dtype="f16", R=50),
+    dict(nq=[130, 0, 300, 65], H=64, kv=8, D=64, dtype="bf16", causal=True, prefix=[0, 0, 70, 65], cap=25.0, R=7),
+    dict(nq=[33, 128, 200], nk=[400, 100, 731], H=64, kv=64, D=128, dtype="f16", causal=True, cap=9.0),
+    dict(nq=[129, 190, 70], nk=[129, 0, 333], H=72, kv=9, D=128, dtype="bf16", R=300),
+]
+FORWARD += WIDE
+
+
 def ident(c):
     return "-".join(f"{k}={v}" for k, v in c.items()).replace(" ", "")
 
@@ -153,6 +163,9 @@ GRAD = [
     dict(nq=[40, 7, 9], nk=[10, 0, 64], H=2, kv=2, D=64, dtype="f16", causal=True, R=5),
     dict(nq=[0, 40], nk=[70, 0], H=2, kv=1, D=64, dtype="bf16", R=5),
 ]
+
+
+GRAD += WIDE[:2] + [dict(nq=[300, 40], H=8, kv=2, D=128, dtype="f16", causal=True, R=900, cap=6.0)]
 
 
 @pytest.mark.parametrize("case", GRAD, ids=ident)
@@ -234,6 +247,18 @@ def test_clips_do_not_reach_each_other():
     keep = [i for i in range(203) if not 100 <= i < 133]
     for n in ("o", "dq", "dk", "dv"):
         ref.check(got[n][keep], want[n][keep], tol[n][keep], n)
+
+
+@pytest.mark.parametrize("cap", [2.0, 5.0])
+def test_scores_far_past_the_cap(cap):
+    """Scores of every size against a small cap: the tanh's three forms, each element of a block by its own."""
+    x = Layer([200], 4, 4, 64, "f16", cap=cap, R=6, scale=0.6)
+    x.q[::3] *= 0.01
+    x.q[1::3] *= 0.2
+    want, tol = x.reference(grad=True)
+    got = x.up().forward(True)
+    for n, y in dict(got, **x.backward()).items():
+        ref.check(y, want[n], tol[n], n)
 
 
 def test_same_results_on_another_stream_and_in_a_graph():

@@ -95,11 +95,10 @@ __device__ __forceinline__ void split8(float16v x, typename Vec8<T>::type (&part
         }
 }
 
-// The largest of three (no operand is a signalling NaN, which fmaxf would see to).
+// The largest of three, NaN if one is.  (A builtin, not assembly: the compiler
+// waits for a matrix product's registers only where it sees them read.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 // Inside an `if` that is rarely taken and the same for the whole wave: keeps the
@@ -114,7 +113,7 @@ __device__ __forceinline__ float max16(const float16v& a) {
     float x = max3(a[0], a[1], a[2]);
 #pragma unroll
     for (int r = 3; r < 15; r += 2) x = max3(x, a[r], a[r + 1]);
-    return fmaxf(x, a[15]);
+    return max3(x, a[15], a[15]);
 }
 
 // ---- LDS tiles of D 16-bit columns, dense rows ----
@@ -248,13 +247,6 @@ __device__ __forceinline__ float tanh_any(float y) {
     return fabsf(y) < 0.5f ? y * horner(y * y, kTanhD) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// The largest of |a|, |b| and c.
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
 // q . k of a block to w, in place.
 template <bool CAP, class V>
 __device__ __forceinline__ void score_w(V& s, const ScoreMap& m) {
@@ -262,14 +254,14 @@ __device__ __forceinline__ void score_w(V& s, const ScoreMap& m) {
         constexpr int N = sizeof(V) / 4;
         float top = 0.0f;
 #pragma unroll
-        for (int r = 0; r < N; r += 2) top = max3_abs(s[r], s[r + 1], top);
+        for (int r = 0; r < N; r += 2) top = max3(fabsf(s[r]), fabsf(s[r + 1]), top);
         auto each = [&](auto f) {
 #pragma unroll
             for (int r = 0; r < N; ++r) s[r] = f(s[r] * m.mul);
         };
-        if (!__any(top > m.lim[0])) {
+        if (!__any(!(top <= m.lim[0]))) {
             each([](float y) { return y * horner(y * y, kTanhC); });
-        } else if (!__any(top > m.lim[1])) {
+        } else if (!__any(!(top <= m.lim[1]))) {
             keep_branch();
             each([](float y) { return y * horner(y * y, kTanhD); });
         } else {

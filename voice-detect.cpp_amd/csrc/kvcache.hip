@@ -172,7 +172,7 @@ __device__ __forceinline__ typename Vec8<T>::type codes8(uint32_t lo, uint32_t h
 // (lds_dst wave-uniform); ordered by the caller's vmcnt waits.
 __device__ __forceinline__ void dma4_lanes(uint8_t* lds_dst, const void* src) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)lds_dst);
-    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0v) : "memory");
 }
 
 // 16-byte chunk c of ring row r: rows of RB bytes, swizzled so that the column
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(PagedArgs a)
         float mx = max3(s[0][0], s[0][1], s[0][2]);
         mx = max3(mx, s[0][3], s[1][0]);
         mx = max3(mx, s[1][1], s[1][2]);
-        mx = fmaxf(mx, s[1][3]);
+        mx = max3(mx, s[1][3], s[1][3]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         if (__any(mx > m + 8.0f)) {

@@ -118,11 +118,11 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
             if constexpr (CAP) {
                 float top = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; r += 2) top = max3_abs(s[r], s[r + 1], top);
-                if (__any(top > a.map.lim[0])) {
+                for (int r = 0; r < 16; r += 2) top = max3(fabsf(s[r]), fabsf(s[r + 1]), top);
+                if (__any(!(top <= a.map.lim[0]))) {
                     keep_branch();
                     poly = 2;
-                    if (__any(top > a.map.lim[1])) {
+                    if (__any(!(top <= a.map.lim[1]))) {
                         keep_branch();
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[r] = am * tanh_any(s[r] * a.map.mul);
@@ -362,8 +362,11 @@ template <class T, int D, bool CAP, bool SPLIT>
 void launch_fwd(const vdk_attn_plan* p, const FwdArgs& a, hipStream_t s) {
     const size_t tab = a.radius ? 4 * (2 * a.radius + 1 + 2 * kTabPad) : 0, wide = 4 * kKeys * D * 2 + tab;
     const size_t narrow = 8 * kKeys * D * 2 + std::max<size_t>(tab, 2048);
-    // below one tile of 128 queries a CU the keys are split as well
-    if ((long long)p->n_q128 * p->n_heads < 256 && narrow <= 163840) launch_tiles<T, D, CAP, SPLIT, true>(p, a, narrow, s);
+    // Few tiles of 128 queries: the keys are split as well.  At 64 dims up to one tile a CU: 24 tiles (149 frames, 12
+    // heads) 6.0 us against 7.3 wide, 288 tiles (6 x 499 frames) 22.7 against 18.1.  At 128 dims, where one such
+    // workgroup fills a CU's LDS, to half of that: 384 tiles 68 us against 33.
+    if ((long long)p->n_q128 * p->n_heads < (D == 64 ? 256 : 128) && narrow <= 163840)
+        launch_tiles<T, D, CAP, SPLIT, true>(p, a, narrow, s);
     else launch_tiles<T, D, CAP, SPLIT, false>(p, a, wide, s);
 }
 
