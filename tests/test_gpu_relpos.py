@@ -165,7 +165,11 @@ GRAD = [
 ]
 
 
-GRAD += WIDE[:2] + [dict(nq=[300, 40], H=8, kv=2, D=128, dtype="f16", causal=True, R=900, cap=6.0)]
+GRAD += WIDE[:2] + [
+    dict(nq=[300, 40], H=8, kv=2, D=128, dtype="f16", causal=True, R=900, cap=6.0),
+    dict(nq=[300, 40, 129], H=16, kv=2, D=128, dtype="f16", causal=True, R=70, cap=25.0),
+    dict(nq=[33, 190, 70], nk=[100, 190, 40], H=16, kv=16, D=128, dtype="bf16", R=30),
+]
 
 
 @pytest.mark.parametrize("case", GRAD, ids=ident)

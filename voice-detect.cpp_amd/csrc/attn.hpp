@@ -309,11 +309,11 @@ void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a);
 }  // namespace vdk
 
 // Work lists: 128 queries and 128 keys an item, heaviest first, and the blocks
-// of 32 queries in order.
+// of 32 queries and of 32 keys in order.
 struct vdk_attn_plan {
     int n_clips, n_heads, n_kv, dim, causal;
     long long total_q, total_kv;
-    int n_q128, n_k128, n_b32;
+    int n_q128, n_k128, n_b32, n_k32;
     void* device;                  // one allocation for all lists
-    vdk::AttnTile *d_q128, *d_k128, *d_b32;
+    vdk::AttnTile *d_q128, *d_k128, *d_b32, *d_k32;
 };

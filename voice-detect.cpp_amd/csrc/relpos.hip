@@ -429,7 +429,7 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         p.dim = head_dim;
         p.causal = causal != 0;
         std::vector<std::pair<long long, AttnTile>> q128, k128;   // (work, tile)
-        std::vector<AttnTile> lists;
+        std::vector<AttnTile> lists, k32;
         int b32 = 0;
         for (int c = 0; c < n_clips; ++c) {
             const long long nq = q_offsets[c + 1] - q_offsets[c], nk = kv_offsets[c + 1] - kv_offsets[c];
@@ -448,8 +448,9 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
                 q128.push_back({seen(std::min(q + 128, nq) - 1), at(q)});
             for (long long q = 0; q < nq; q += 32) lists.push_back(at(q));
             b32 += cdiv(nq, 32);
-            require((long long)b32 * n_heads < (1 << 30) && k128.size() * n_heads < (1u << 30),
+            require((long long)b32 * n_heads < (1 << 30) && k32.size() * n_heads < (1u << 30),
                     "attn_plan: too many tiles for one launch");
+            for (long long k = 0; k < nk; k += 32) k32.push_back(at(k));
             for (long long k = 0; k < nk; k += 128) {
                 const long long first = p.causal && k >= pre ? std::max(0ll, k - past) : 0;   // the first query that sees it
                 k128.push_back({std::max(0ll, nq - first), at(k)});
@@ -465,12 +466,15 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         p.n_q128 = (int)q128.size();
         p.n_k128 = (int)k128.size();
         p.n_b32 = b32;
+        p.n_k32 = (int)k32.size();
+        lists.insert(lists.end(), k32.begin(), k32.end());
         const size_t bytes = lists.size() * sizeof(AttnTile);
         if (vdk_device_count() > 0 && bytes > 0) {
             VDK_HIP(hipMalloc(&p.device, bytes));
             p.d_b32 = static_cast<AttnTile*>(p.device);
             p.d_q128 = p.d_b32 + p.n_b32;
             p.d_k128 = p.d_q128 + p.n_q128;
+            p.d_k32 = p.d_k128 + p.n_k128;
             try {
                 VDK_HIP(hipMemcpy(p.device, lists.data(), bytes, hipMemcpyHostToDevice));
                 *plan = new vdk_attn_plan(p);

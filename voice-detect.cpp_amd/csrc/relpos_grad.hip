@@ -26,10 +26,10 @@ struct GradArgs {
     float scale;
     void *dq, *dk, *dv;
     long long dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
-    float *delta, *most, *part, *d_dist;   // [heads][total_q], [heads][blocks], [heads][blocks][2 R + 1], the result
-    int2* span;                            // [blocks]: the distances a block of 32 queries has written
+    float *delta, *most, *part, *d_dist;   // [heads][total_q], [heads][blocks], [heads][rows][2 R + 1], the result
+    int2* span;                            // [rows]: the distances that a wave of 32 queries has written
     const AttnTile *q_tiles, *k_tiles, *blocks;
-    int n_q, n_k, n_heads, n_kv, group, causal, n_b32;
+    int n_q, n_k, n_heads, n_kv, group, causal, n_b32, n_rows;
     long long total_q, total_kv;
     float* kv_part;                        // [head_parts][2][total_kv][n_kv][D], where the heads of a key head are split
     int head_parts;
@@ -112,20 +112,20 @@ __global__ __launch_bounds__(256) void relpos_delta_kernel(GradArgs a) {
 }
 
 // dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32.
-template <class T, int D, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS, bool NARROW>
 __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
-    constexpr int NW = 4, kTile = kKeys * D * 2;
+    constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2, kBlock = NARROW ? 32 : 64;   // (a wave's keys of a step)
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
     const int2 ht = head_tile(bid, a.n_q, a.n_heads);
     const int h = ht.x;
     const AttnTile c = a.q_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, qw = c.row + 32 * wave, qi = qw + lr;
+    const int past = c.nk - c.nq, qw = c.row + (NARROW ? 0 : 32 * wave), qi = qw + lr;
     const int qr = qi < c.nq ? qi : c.nq - 1;
     auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
-    const int kend = max(last(min(c.row + 32 * NW, c.nq) - 1), 0);
+    const int kend = max(last(min(c.row + (NARROW ? 32 : 32 * NW), c.nq) - 1), 0);
     const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
     const int kfull = qw < c.nq ? last(qw) : 0;
     const int lim = last(qr);
@@ -133,7 +133,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     const uint32_t kb_row = (uint32_t)a.k_tok * 2, vb_row = (uint32_t)a.v_tok * 2;
     const T* kp = static_cast<const T*>(a.k) + c.k0 * a.k_tok + (long long)(h / a.group) * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + c.k0 * a.v_tok + (long long)(h / a.group) * a.v_head;
-    TileDma<D, kKeys, NW> dk, dv;
+    TileDma<D, kStep, NW> dk, dv;
     dk.init(kb_row, wave, lane);
     dv.init(vb_row, wave, lane);
     auto fetch = [&](int kb, int buf) {
@@ -175,17 +175,19 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     float acc[5] = {0, 0, 0, 0, 0}, left = 0.0f, right = 0.0f;
     int lo = 1 << 30, hi = -(1 << 30);
     float* part = nullptr;
+    const int row = NARROW ? 4 * (c.b32 + (qw >> 5)) + wave : c.b32 + (qw >> 5);
     if constexpr (BIAS) {
-        part = a.part + ((long long)h * a.n_b32 + c.b32 + (qw >> 5)) * (2 * R + 1);
+        part = a.part + ((long long)h * a.n_rows + row) * (2 * R + 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ring[64 * i + lane] = 0.0f;
     }
     // acc[0..3] hold all that their 16 lanes add to the 64 distances from d0 - 15 (+ 4 hl - 16 (lr / 16)): stored, and
-    // the 64 distances from d0 - 31, which no later tile reaches, summed over the four sixteens and written out
+    // the 64 distances from d0 - 31, which no later tile reaches, summed over the four sixteens and written out.
+    // (NARROW: a wave's blocks lie 128 distances apart, so each is written whole, zeros up to the next.)
     auto flush = [&](int d0) {
         const int rho = lane >> 4, off = 4 * hl - 16 * (rho & 1) - (lane & 15);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ring[128 * rho + ((d0 + off + 16 * j) & 127)] = acc[j];
+        for (int j = 0; j < (NARROW ? 5 : 4); ++j) ring[128 * rho + ((d0 + off + 16 * j) & 127)] = acc[j];
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         const int d = d0 - 31 + lane;
@@ -197,7 +199,8 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
         if (d <= -R) left += v;
         else if (d >= R) right += v;
         else part[d + R] = v;
-        acc[0] = acc[4];
+        if (NARROW && d + 64 > -R && d + 64 < R) part[d + 64 + R] = 0.0f;
+        acc[0] = NARROW ? 0.0f : acc[4];
         acc[1] = acc[2] = acc[3] = acc[4] = 0.0f;
     };
 
@@ -206,19 +209,20 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     for (int dt = 0; dt < D / 32; ++dt) dq[dt] = splat16(0.0f);
     const float am = a.map.am;
     TileReads<T, D> at;
-    at.init(smem, lane);
+    at.init(smem + (NARROW ? wave * (64 * D) : 0), lane);
     const float unscale = kScaled<T> ? 1.0f / sc * 0x1p-8f : 1.0f;   // of dS, per row (a power of two)
-    for (int kb = 0, buf = 0; kb < kend; kb += kKeys, buf ^= 1) {
+    for (int k0 = 0, buf = 0; k0 < kend; k0 += kStep, buf ^= 1) {
         wait_vmcnt<0>();
         lds_barrier();
-        if (kb + kKeys < kend) fetch(kb + kKeys, buf ^ 1);
+        if (k0 + kStep < kend) fetch(k0 + kStep, buf ^ 1);
+        const int kb = k0 + (NARROW ? 32 * wave : 0);
         if (kb >= kend_w) continue;
         const int tk = buf * 2 * kTile, tv = tk + kTile;
         const int d0 = kb - (qw + past);
-        const bool near = BIAS && d0 + 63 > -R && d0 - 31 < R;
+        const bool near = BIAS && d0 + kBlock - 1 > -R && d0 - 31 < R;
         const float add = (d0 < 0 ? far_l : far_r) - L2;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < kBlock / 32; ++kt) {
             float16v s = splat16(0.0f), p = splat16(0.0f);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tk, kt, kk), qf[kk], s);
@@ -235,7 +239,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], am, add));
             }
-            if (kb + kKeys > kfull) {
+            if (kb + kBlock > kfull) {
                 keep_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -276,7 +280,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
                 lo = min(lo, d0 - 31);
                 hi = d0 + 96;
                 flush(d0);
-                if (kb + kKeys >= kend_w || d0 + 64 - 31 >= R) flush(d0 + 64);   // the last one: what is left
+                if (!NARROW && (kb + kKeys >= kend_w || d0 + 64 - 31 >= R)) flush(d0 + 64);   // the last one: what is left
             }
         }
     }
@@ -290,44 +294,60 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
             if (lane == 0) {
                 part[0] = left;
                 part[2 * R] = right;
-                if (h == 0) a.span[c.b32 + (qw >> 5)] = int2{lo, hi};
+                if (h == 0) a.span[row] = int2{lo, hi};
             }
         }
+    }
+    float* js = reinterpret_cast<float*>(smem);   // [wave][register][lane]
+    if constexpr (NARROW) {
+        __syncthreads();   // the tiles are no longer read
+#pragma unroll
+        for (int r = 0; r < D / 2; ++r) js[(wave * (D / 2) + r) * 64 + lane] = dq[r >> 4][r & 15];
+        __syncthreads();
     }
     if (qi >= c.nq) return;
     const float f = a.scale * 0x1p-8f / sc;   // undo 2^8 and sc (both powers of two)
     T* out = static_cast<T*>(a.dq) + (c.q0 + qi) * a.dq_tok + (long long)h * a.dq_head;
+    constexpr int kOut = NARROW ? D / 32 : D / 8;   // a wave's groups of four registers
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int j = 0; j < kOut; ++j) {
+        const int i = NARROW ? wave * kOut + j : j;
+        float4v v = {0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const auto u0 = pack2<T>(dq[dt][4 * g] * f, dq[dt][4 * g + 1] * f),
-                       u1 = pack2<T>(dq[dt][4 * g + 2] * f, dq[dt][4 * g + 3] * f);
-            *reinterpret_cast<uint2*>(out + 32 * dt + 8 * g + 4 * hl) =
-                uint2{__builtin_bit_cast(uint32_t, u0), __builtin_bit_cast(uint32_t, u1)};
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (NARROW) {
+#pragma unroll
+                for (int w = 0; w < NW; ++w) v[e] += js[(w * (D / 2) + 4 * i + e) * 64 + lane];
+            } else {
+                v[e] = dq[j >> 2][4 * (j & 3) + e];
+            }
         }
+        *reinterpret_cast<uint2*>(out + 32 * (i >> 2) + 8 * (i & 3) + 4 * hl) =
+            uint2{__builtin_bit_cast(uint32_t, pack2<T>(v[0] * f, v[1] * f)),
+                  __builtin_bit_cast(uint32_t, pack2<T>(v[2] * f, v[3] * f))};
+    }
 }
 
 // dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 queries a step
 // through LDS, the heads that share the keys one after the other, or a part of
 // them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
-template <class T, int D, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS, bool NARROW>
 __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
-    constexpr int NW = 4, kTile = kKeys * D * 2;
-    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][64]: -L2 (without a cap by am) and -delta of a step's queries
-    float* tab = rows + 256;
+    constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
+    float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][kStep]: -L2 (without a cap by am) and -delta of a step's queries
+    float* tab = rows + 4 * kStep;
     const int2 ht = head_tile(bid, a.n_k, a.n_kv * a.head_parts);
     const int kvh = ht.x / a.head_parts, hp = ht.x - kvh * a.head_parts;
     const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
     const AttnTile c = a.k_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, kw = c.row + 32 * wave, ki = kw + lr;
+    const int past = c.nk - c.nq, kw = c.row + (NARROW ? 0 : 32 * wave), ki = kw + lr;
     const int kr = ki < c.nk ? ki : c.nk - 1;
     // the first query that sees a key of the tile, down to a whole step
     const int q_first = a.causal && c.row >= c.prefix ? max(c.row - past, 0) & ~63 : 0;
-    const int per_head = q_first < c.nq ? (c.nq - q_first + 63) >> 6 : 0, steps = per_head * heads;
+    const int per_head = q_first < c.nq ? (c.nq - q_first + kStep - 1) / kStep : 0, steps = per_head * heads;
 
     const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + (c.k0 + kr) * a.v_tok + (long long)kvh * a.v_head;
@@ -338,25 +358,29 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         vf[kk] = *reinterpret_cast<const V8*>(vp + 16 * kk + 8 * hl);
     }
     const uint32_t qb_row = (uint32_t)a.q_tok * 2, db_row = (uint32_t)a.do_tok * 2;
-    TileDma<D, kKeys, NW> dmq, dmo;
+    TileDma<D, kStep, NW> dmq, dmo;
     dmq.init(qb_row, wave, lane);
     dmo.init(db_row, wave, lane);
     float row_v = 0.0f;   // this thread's entry of the next step's rows[]
-    auto step_scale = [&](int h, int q) {   // from the step's largest |dO|
+    auto step_scale = [&](int h, int q) {   // from the largest |dO| of the step's (the wave's) queries
         if constexpr (!kScaled<T>) return 1.0f;
+        if constexpr (NARROW) {
+            q += 32 * wave;
+            return q < c.nq ? scale_of(a.most[h * a.n_b32 + c.b32 + (q >> 5)]) : 1.0f;
+        }
         const float* p = a.most + h * a.n_b32 + c.b32 + (q >> 5);
         return scale_of(q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
     };
     auto fetch = [&](int it, int buf) {
-        const int h = h0 + it / per_head, q = q_first + (it % per_head) * 64;
+        const int h = h0 + it / per_head, q = q_first + (it % per_head) * kStep;
         const T* qs = static_cast<const T*>(a.q) + (c.q0 + q) * a.q_tok + (long long)h * a.q_head;
         const T* ds = static_cast<const T*>(a.d_o) + (c.q0 + q) * a.do_tok + (long long)h * a.do_head;
         dmq.load(smem + buf * 2 * kTile, qs, qb_row, c.nq - q, wave);
         dmo.load(smem + buf * 2 * kTile + kTile, ds, db_row, c.nq - q, wave);
-        if (threadIdx.x < 128) {
-            const int qi = q + (threadIdx.x & 63);
+        if (threadIdx.x < 2 * kStep) {
+            const int qi = q + (threadIdx.x & (kStep - 1));
             const long long at = h * a.total_q + c.q0 + min(qi, c.nq - 1);
-            if (threadIdx.x < 64) {
+            if (threadIdx.x < kStep) {
                 const float lse = a.lse[at];
                 row_v = qi < c.nq && !(lse < -1e30f) ? (kPShift - lse * kLog2e) * (CAP ? 1.0f : 1.0f / a.map.am) : -FLT_MAX;
             } else {
@@ -372,13 +396,13 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = splat16(0.0f);
     const float am = a.map.am;
     TileReads<T, D> at;
-    at.init(smem, lane);
+    at.init(smem + (NARROW ? wave * (64 * D) : 0), lane);
     float sc = 1.0f, far_l = 0.0f, far_r = 0.0f;
     if constexpr (kScaled<T>) {
         if (steps > 0) sc = step_scale(h0, q_first);
     }
     for (int it = 0, buf = 0; it < steps; ++it, buf ^= 1) {
-        const int h = h0 + it / per_head, q = q_first + (it % per_head) * 64;
+        const int h = h0 + it / per_head, q = q_first + (it % per_head) * kStep;
         if constexpr (BIAS) {
             if (it % per_head == 0) {   // another head's bias
                 lds_barrier();
@@ -389,11 +413,11 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
                 far_r = bias2_of(b[2 * R]);
             }
         }
-        if (threadIdx.x < 128) rows[buf * 128 + threadIdx.x] = row_v;
+        if (threadIdx.x < 2 * kStep) rows[buf * 2 * kStep + threadIdx.x] = row_v;
         wait_vmcnt<0>();
         lds_barrier();
-        const float* nl = rows + buf * 128;
-        const float* nd = nl + 64;
+        const float* nl = rows + buf * 2 * kStep + (NARROW ? 32 * wave : 0);
+        const float* nd = nl + kStep;
         if (it + 1 < steps) fetch(it + 1, buf ^ 1);
         if constexpr (kScaled<T>) {   // dK is carried in the scale of the step: moved with it, exactly
             const float s_new = step_scale(h, q);
@@ -408,8 +432,8 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         }
         const int tq = buf * 2 * kTile, to = tq + kTile;
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
-            const int qs = q + 32 * qt;
+        for (int qt = 0; qt < (NARROW ? 1 : 2); ++qt) {
+            const int qs = q + 32 * (NARROW ? wave : qt);
             if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
             // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki.  The sums start from the rows' own terms
             float16v s, p;
@@ -476,52 +500,55 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
             }
         }
     }
-    if (ki >= c.nk) return;
     const float f = a.scale * 0x1p-8f / sc;
-    if (a.head_parts > 1) {
-        float* out = a.kv_part + (((long long)hp * 2 * a.total_kv + c.k0 + ki) * a.n_kv + kvh) * D;
+    float* js = reinterpret_cast<float*>(smem);   // [wave][dK's and dV's registers][lane]
+    if constexpr (NARROW) {
+        __syncthreads();   // the tiles are no longer read
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float4v k4, v4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    k4[e] = dk[dt][4 * g + e] * f;
-                    v4[e] = dv[dt][4 * g + e] * 0x1p-8f;
-                }
-                float* at = out + 32 * dt + 8 * g + 4 * hl;
-                *reinterpret_cast<float4v*>(at) = k4;
-                *reinterpret_cast<float4v*>(at + a.total_kv * a.n_kv * D) = v4;
-            }
-        return;
+        for (int r = 0; r < D / 2; ++r) {
+            js[(wave * D + r) * 64 + lane] = dk[r >> 4][r & 15] * f;   // (each wave's own scale)
+            js[(wave * D + D / 2 + r) * 64 + lane] = dv[r >> 4][r & 15] * 0x1p-8f;
+        }
+        __syncthreads();
     }
+    if (ki >= c.nk) return;
+    float* parts = a.kv_part + (((long long)hp * 2 * a.total_kv + c.k0 + ki) * a.n_kv + kvh) * D;
     T* ok = static_cast<T*>(a.dk) + (c.k0 + ki) * a.dk_tok + (long long)kvh * a.dk_head;
     T* ov = static_cast<T*>(a.dv) + (c.k0 + ki) * a.dv_tok + (long long)kvh * a.dv_head;
+    constexpr int kOut = NARROW ? D / 16 : D / 4;   // a wave's groups of four registers, dK's and dV's
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int j = 0; j < kOut; ++j) {
+        const int i = NARROW ? wave * kOut + j : j, of = i >= D / 8, g = of ? i - D / 8 : i;
+        float4v v = {0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = 32 * dt + 8 * g + 4 * hl;
-            auto put = [&](T* out, const float16v& x, float m) {
-                const auto u0 = pack2<T>(x[4 * g] * m, x[4 * g + 1] * m), u1 = pack2<T>(x[4 * g + 2] * m, x[4 * g + 3] * m);
-                *reinterpret_cast<uint2*>(out + d) =
-                    uint2{__builtin_bit_cast(uint32_t, u0), __builtin_bit_cast(uint32_t, u1)};
-            };
-            put(ok, dk[dt], f);
-            put(ov, dv[dt], 0x1p-8f);
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (NARROW) {
+#pragma unroll
+                for (int w = 0; w < NW; ++w) v[e] += js[(w * D + 4 * i + e) * 64 + lane];
+            } else {
+                v[e] = j < D / 8 ? dk[(j >> 2) % (D / 32)][4 * (j & 3) + e] * f : dv[(j >> 2) % (D / 32)][4 * (j & 3) + e] * 0x1p-8f;
+            }
         }
+        const int d = 32 * (g >> 2) + 8 * (g & 3) + 4 * hl;
+        if (a.head_parts > 1) {
+            *reinterpret_cast<float4v*>(parts + (of ? a.total_kv * a.n_kv * D : 0) + d) = v;
+        } else {
+            *reinterpret_cast<uint2*>((of ? ov : ok) + d) = uint2{__builtin_bit_cast(uint32_t, pack2<T>(v[0], v[1])),
+                                                                   __builtin_bit_cast(uint32_t, pack2<T>(v[2], v[3]))};
+        }
+    }
 }
 
 // Both in one launch, the longer tiles of dK and dV first: the tiles of one fill the chip while the other's last ones run.
-template <class T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
+// NARROW: 32 queries (keys) a workgroup, whose waves share its keys (queries).
+template <class T, int D, bool CAP, bool BIAS, bool NARROW>
+__global__ __launch_bounds__(256, D == 128 ? 1 : NARROW ? 2 : 3) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int b = blockIdx.x;
     if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
-        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS>(a, b, smem);
+        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS, NARROW>(a, b, smem);
     } else {
-        dq_tile<T, D, CAP, BIAS>(a, b - n_dkv8, smem);
+        dq_tile<T, D, CAP, BIAS, NARROW>(a, b - n_dkv8, smem);
     }
 }
 
@@ -550,11 +577,27 @@ __global__ __launch_bounds__(256) void relpos_dkv_join_kernel(GradArgs a) {
     *reinterpret_cast<typename Vec8<T>::type*>(out + d) = v;
 }
 
-// How many parts the heads of a key head are cut into: 1024 workgroups fill the
-// chip twice, and causal tiles differ most in their work where they are few.
-int head_parts_of(const vdk_attn_plan* p) {
-    const long long groups = std::max(1ll, (long long)p->n_k128 * p->n_kv);
-    return (int)std::max(1ll, std::min<long long>(p->n_heads / p->n_kv, (1024 + groups - 1) / groups));
+// How a layout's backward pass is cut.
+struct GradCut {
+    bool narrow;
+    int head_parts;    // workgroups that share the heads of a key head
+    int lds, rows;     // rows of partial sums of the bias's gradient
+};
+
+GradCut cut_of(const vdk_attn_plan* p, int radius) {
+    const int bias = radius ? 4 * (2 * radius + 1 + 2 * kTabPad) + 16 + 4 * 512 * 4 : 0;
+    const int narrow = 8 * kKeys * p->dim * 2 + 2048 + bias, wide = 4 * kKeys * p->dim * 2 + 1024 + bias;
+    GradCut c;
+    // Smaller tiles where those of 128 queries leave most CUs idle.  At 64 dims to one for every second CU: 96 tiles (one
+    // clip of 1500, 8 heads) 60 us against 73, 48 tiles 103 against 141; 240 tiles of short clips 39 against 30.  At 128
+    // dims, where one workgroup fills a CU's LDS, far fewer: 32 tiles 77 us against 119, 60 tiles 135 against 111.
+    c.narrow = (long long)p->n_q128 * p->n_heads <= (p->dim == 64 ? 128 : 32) && narrow <= 163840;
+    c.lds = c.narrow ? narrow : wide;
+    c.rows = p->n_b32 * (c.narrow ? 4 : 1);
+    // 1024 workgroups (narrow: 512) fill the chip twice, and causal tiles differ most in their work where they are few
+    const long long groups = std::max(1ll, (long long)(c.narrow ? p->n_k32 : p->n_k128) * p->n_kv);
+    c.head_parts = (int)std::max(1ll, std::min<long long>(p->n_heads / p->n_kv, ((c.narrow ? 512 : 1024) + groups - 1) / groups));
+    return c;
 }
 
 // The blocks' partial sums of 64 distances, 16 rows of blocks at a time, in a fixed order.
@@ -564,14 +607,14 @@ __global__ __launch_bounds__(1024) void relpos_dbias_kernel(GradArgs a) {
     double sum = 0.0;
     if (i <= 2 * R) {
         const bool edge = i == 0 || i == 2 * R;
-        const float* p = a.part + (long long)h * a.n_b32 * (2 * R + 1) + i;
-        for (int b0 = row; b0 < a.n_b32; b0 += 16 * 8) {   // eight loads at a time
+        const float* p = a.part + (long long)h * a.n_rows * (2 * R + 1) + i;
+        for (int b0 = row; b0 < a.n_rows; b0 += 16 * 8) {   // eight loads at a time
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int b = min(b0 + 16 * j, a.n_b32 - 1);
+                const int b = min(b0 + 16 * j, a.n_rows - 1);
                 const int2 s = a.span[b];
-                const bool ok = b0 + 16 * j < a.n_b32 && (edge || (i - R >= s.x && i - R <= s.y));
+                const bool ok = b0 + 16 * j < a.n_rows && (edge || (i - R >= s.x && i - R <= s.y));
                 v[j] = ok ? p[(long long)b * (2 * R + 1)] : 0.0f;
             }
 #pragma unroll
@@ -591,7 +634,7 @@ __global__ __launch_bounds__(1024) void relpos_dbias_kernel(GradArgs a) {
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 template <class T, int D, bool CAP, bool BIAS>
-void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
+void launch_grad(const vdk_attn_plan* p, GradArgs a, const GradCut& cut, hipStream_t s) {
     if (p->n_b32) {
         hipLaunchKernelGGL((relpos_delta_kernel<T, D>), dim3(p->n_b32, a.n_heads), dim3(256), 0, s, a);
         VDK_HIP(hipGetLastError());
@@ -599,11 +642,10 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
     const long long n_dkv = (long long)a.n_k * a.n_kv * a.head_parts, n_dkv8 = (n_dkv + 7) / 8 * 8;
     const long long n = n_dkv8 + (long long)a.n_q * a.n_heads;
     if (n > 0) {
-        auto kern = relpos_grad_kernel<T, D, CAP, BIAS>;
-        const int lds = 4 * kKeys * D * 2 + 1024 + (BIAS ? 4 * (2 * a.radius + 1 + 2 * kTabPad) + 16 + 4 * 512 * 4 : 0);
-        if (lds > 65536)
-            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), lds, s, a, (int)n_dkv, (int)n_dkv8);
+        auto kern = cut.narrow ? relpos_grad_kernel<T, D, CAP, BIAS, true> : relpos_grad_kernel<T, D, CAP, BIAS, false>;
+        if (cut.lds > 65536)
+            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, cut.lds));
+        hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), cut.lds, s, a, (int)n_dkv, (int)n_dkv8);
         VDK_HIP(hipGetLastError());
         if (a.head_parts > 1) {
             const long long threads = a.total_kv * a.n_kv * (D / 8);
@@ -618,9 +660,9 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, hipStream_t s) {
 }
 
 template <class T, int D>
-void launch_grad_t(const vdk_attn_plan* p, const GradArgs& a, bool cap, hipStream_t s) {
-    if (a.radius) cap ? launch_grad<T, D, true, true>(p, a, s) : launch_grad<T, D, false, true>(p, a, s);
-    else cap ? launch_grad<T, D, true, false>(p, a, s) : launch_grad<T, D, false, false>(p, a, s);
+void launch_grad_t(const vdk_attn_plan* p, const GradArgs& a, bool cap, const GradCut& c, hipStream_t s) {
+    if (a.radius) cap ? launch_grad<T, D, true, true>(p, a, c, s) : launch_grad<T, D, false, true>(p, a, c, s);
+    else cap ? launch_grad<T, D, true, false>(p, a, c, s) : launch_grad<T, D, false, false>(p, a, c, s);
 }
 
 }  // namespace
@@ -633,11 +675,11 @@ extern "C" size_t vdk_relpos_attention_backward_workspace_size(const vdk_attn_pl
     if (guarded([&] {
             require(p, "relpos_attention_backward: NULL plan");
             require(bias_radius >= 0 && bias_radius <= 4096, "relpos_attention_backward: bias_radius must be 0 .. 4096");
-            const int parts = head_parts_of(p);
-            n = parts > 1 ? (size_t)parts * 2 * p->total_kv * p->n_kv * p->dim * 4 : 0;
+            const GradCut cut = cut_of(p, bias_radius);
+            n = cut.head_parts > 1 ? (size_t)cut.head_parts * 2 * p->total_kv * p->n_kv * p->dim * 4 : 0;
             n += up16((size_t)p->n_heads * p->total_q * 4) + up16((size_t)p->n_heads * p->n_b32 * 4) +
-                up16((size_t)p->n_b32 * sizeof(int2)) +
-                (bias_radius ? (size_t)p->n_heads * p->n_b32 * (2 * bias_radius + 1) * 4 : 0);
+                up16((size_t)cut.rows * sizeof(int2)) +
+                (bias_radius ? (size_t)p->n_heads * cut.rows * (2 * bias_radius + 1) * 4 : 0);
         }) != 0)
         return 0;
     return up16(n);
@@ -680,17 +722,19 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
         f.most = reinterpret_cast<float*>(w);
         w += up16((size_t)p->n_heads * p->n_b32 * 4);
         f.span = reinterpret_cast<int2*>(w);
-        w += up16((size_t)p->n_b32 * sizeof(int2));
-        f.head_parts = head_parts_of(p);
+        const GradCut cut = cut_of(p, R);
+        w += up16((size_t)cut.rows * sizeof(int2));
+        f.n_rows = cut.rows;
+        f.head_parts = cut.head_parts;
         f.kv_part = reinterpret_cast<float*>(w);
         if (f.head_parts > 1) w += (size_t)f.head_parts * 2 * p->total_kv * p->n_kv * p->dim * 4;
         f.part = reinterpret_cast<float*>(w);
         f.d_dist = g->d_dist_bias;
-        f.q_tiles = p->d_q128;
-        f.k_tiles = p->d_k128;
+        f.q_tiles = cut.narrow ? p->d_b32 : p->d_q128;
+        f.k_tiles = cut.narrow ? p->d_k32 : p->d_k128;
         f.blocks = p->d_b32;
-        f.n_q = p->n_q128;
-        f.n_k = p->n_k128;
+        f.n_q = cut.narrow ? p->n_b32 : p->n_q128;
+        f.n_k = cut.narrow ? p->n_k32 : p->n_k128;
         f.n_heads = p->n_heads;
         f.n_kv = p->n_kv;
         f.group = p->n_heads / p->n_kv;
@@ -699,9 +743,9 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
         f.total_q = p->total_q;
         f.total_kv = p->total_kv;
         hipStream_t s = static_cast<hipStream_t>(stream);
-        if (a->dtype == VDK_F16) p->dim == 64 ? launch_grad_t<half_t, 64>(p, f, a->cap > 0, s)
-                                              : launch_grad_t<half_t, 128>(p, f, a->cap > 0, s);
-        else p->dim == 64 ? launch_grad_t<bf16_t, 64>(p, f, a->cap > 0, s)
-                          : launch_grad_t<bf16_t, 128>(p, f, a->cap > 0, s);
+        if (a->dtype == VDK_F16) p->dim == 64 ? launch_grad_t<half_t, 64>(p, f, a->cap > 0, cut, s)
+                                              : launch_grad_t<half_t, 128>(p, f, a->cap > 0, cut, s);
+        else p->dim == 64 ? launch_grad_t<bf16_t, 64>(p, f, a->cap > 0, cut, s)
+                          : launch_grad_t<bf16_t, 128>(p, f, a->cap > 0, cut, s);
     });
 }

@@ -21,6 +21,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from vdamd import lib
 
 LENGTHS, HEADS, KV, DIM, RADIUS, BUCKETS, FAR, CAP, PAGE = [150, 61, 97], 8, 4, 64, 64, 16, 64, 30.0, 32
+RATE = 1.0   # of the mean gradient of a frame
 
 
 def half(rng, *shape):
@@ -127,7 +128,7 @@ def main():
     for _ in range(30):
         o = layer.forward(table)
         losses.append(float(0.5 * ((o - target) ** 2).sum() / n))
-        table -= 0.05 * layer.backward(o - target)
+        table -= RATE * layer.backward(o - target) / n
     print(f"training the position bias: loss {losses[0]:.4f} -> {losses[-1]:.4f} in {len(losses)} steps")
 
     packed = layer.forward(table)
