@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import attn_ref as ref
+from attn_gpu import Dev, bits, full
 from gpu_util import announce, device_ok
 from vdamd import lib
 
@@ -17,37 +18,48 @@ class Cache:
     def __init__(self, pages, page, kv, D, dtype, quant, fill=None):
         self.t, self.quant, self.page, self.kv, self.D, self.pages = TYPES[dtype], quant, page, kv, D, pages
         shape = (pages, kv, page, D)
-        self.k, self.v = ((torch.full(shape, 0x7f if fill else 0, dtype=torch.uint8, device="cuda") if quant else
-                           torch.full(shape, float("nan") if fill else 0.0, dtype=self.t, device="cuda")) for _ in range(2))
-        self.ks, self.vs = ((torch.full(shape[:3], float("nan") if fill else 0.0, device="cuda") if quant else None)
-                            for _ in range(2))
-        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.k, self.v = ((full(shape, 0x7f if fill else 0, torch.uint8) if quant else
+                           full(shape, float("nan") if fill else 0.0, self.t)) for _ in range(2))
+        self.ks, self.vs = ((full(shape[:3], float("nan") if fill else 0.0) if quant else None) for _ in range(2))
+        self.status = full((1,), 0, torch.int32)
         d = self.d = lib.KvCache()
         d.dtype, d.format = (lib.F16 if dtype == "f16" else lib.BF16), (lib.KV_E4M3 if quant else lib.KV_16)
         d.n_pages, d.page_size, d.n_kv_heads, d.head_dim = pages, page, kv, D
-        d.k, d.v = self.k.data_ptr(), self.v.data_ptr()
+        d.k, d.v = self.k.ptr, self.v.ptr
         if quant:
-            d.k_scale, d.v_scale = self.ks.data_ptr(), self.vs.data_ptr()
+            d.k_scale, d.v_scale = self.ks.ptr, self.vs.ptr
 
     def write(self, slots, k, v):
-        s = slots.cuda()
-        lib.check(lib.lib().vdk_kv_cache_write(self.d, s.data_ptr(), len(slots), k.data_ptr(), k.stride(0), k.stride(1),
-                                               v.data_ptr(), v.stride(0), v.stride(1), self.status.data_ptr(), None))
-        torch.cuda.synchronize()
+        """k and v [n][kv][D], given as halves of one buffer."""
+        s, both, tok = Dev(slots), Dev(torch.cat([k, v], 1)), 2 * self.kv * self.D
+        lib.check(lib.lib().vdk_kv_cache_write(self.d, s.ptr, len(slots), both.ptr, tok, self.D, both.at(self.kv * self.D),
+                                               tok, self.D, self.status.ptr, None))
+        lib.check(lib.lib().vdk_synchronize())
 
     def read(self, slots):
-        s = slots.cuda()
-        k, v = (torch.full((len(slots), self.kv + 1, self.D), 7.0, dtype=self.t, device="cuda") for _ in range(2))
-        lib.check(lib.lib().vdk_kv_cache_read(self.d, s.data_ptr(), len(slots), k.data_ptr(), k.stride(0), k.stride(1),
-                                              v.data_ptr(), v.stride(0), v.stride(1), self.status.data_ptr(), None))
-        torch.cuda.synchronize()
+        s, tok = Dev(slots), (self.kv + 1) * self.D
+        k, v = (full((len(slots), self.kv + 1, self.D), 7.0, self.t) for _ in range(2))
+        lib.check(lib.lib().vdk_kv_cache_read(self.d, s.ptr, len(slots), k.ptr, tok, self.D, v.ptr, tok, self.D,
+                                              self.status.ptr, None))
+        k, v = k.get(), v.get()
         assert (k[:, self.kv] == 7).all() and (v[:, self.kv] == 7).all()
         return k[:, :self.kv], v[:, :self.kv]
 
     def flags(self):
-        x = int(self.status.item())
-        self.status.zero_()
+        x = int(self.status.get())
+        self.status.put(torch.zeros(1, dtype=torch.int32))
         return x
+
+    def held(self, slots):
+        """The rows' values as the cache holds them, in 64 bits: codes times scales."""
+        out = []
+        for x, sc in ((self.k, self.ks), (self.v, self.vs)):
+            x = x.get()[slots // self.page, :, slots % self.page]
+            if self.quant:
+                x = x.view(torch.float8_e4m3fn).float().double() \
+                    * sc.get()[slots // self.page, :, slots % self.page].double()[..., None]
+            out.append(x.double())
+        return tuple(out)
 
 
 def e4m3(y):
@@ -72,35 +84,35 @@ def test_rows_written_and_read_back(n, page, kv, D, dtype, quant):
         kv2[2] *= 2.0 ** 7
         kv2[3, 0] = 0.0
         kv2[3, 0, 5] = 2.0 ** -14
-    both = kv2.to(TYPES[dtype]).cuda()
+    both = kv2.to(TYPES[dtype])
     k, v = both[:, :kv], both[:, kv:]
     slots = torch.randperm(pages * page, generator=g)[:n]
     c.write(slots, k, v)
     back = c.read(slots)
     assert c.flags() == 0
     for x, y, held, scales in ((k, back[0], c.k, c.ks), (v, back[1], c.v, c.vs)):
-        rows = x.double().cpu()
+        rows, held = x.double(), held.get()
         if not quant:
             assert torch.equal(y, x)
             assert torch.equal(held[slots // page, :, slots % page], x)
             continue
         m = rows.abs().amax(-1, keepdim=True).clamp_min(2.0 ** -64)
         code = e4m3(rows * 448 / m)
-        got = held[slots // page, :, slots % page].view(torch.float8_e4m3fn).float().double().cpu()
+        got = held[slots // page, :, slots % page].view(torch.float8_e4m3fn).float().double()
         assert torch.equal(got, code)
-        scale = scales[slots // page, :, slots % page].cpu()
+        scale = scales.get()[slots // page, :, slots % page]
         assert torch.equal(scale, (m.float() / 448).squeeze(-1))
-        assert torch.equal(y.cpu(), (code.float() * scale[..., None]).to(x.dtype))
+        assert torch.equal(y, (code.float() * scale[..., None]).to(x.dtype))
     other = torch.ones(pages * page, dtype=torch.bool)
     other[slots] = False
     untouched = torch.arange(pages * page)[other]
-    assert (c.k[untouched // page, :, untouched % page].float() == 0).all()
+    assert (c.k.get()[untouched // page, :, untouched % page].float() == 0).all()
 
 
 @pytest.mark.parametrize("quant", [True, False], ids=["e4m3", "16"])
 def test_skipped_and_bad_slots_and_rows_that_are_not_finite(quant):
     c = Cache(2, 16, 2, 64, "f16", quant)
-    x = torch.randn(6, 2, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    x = torch.randn(6, 2, 64, generator=torch.Generator().manual_seed(1)).half()
     x[2, 0, 3], x[3, 1, 63] = float("inf"), float("nan")
     slots = torch.tensor([5, -1, 6, 7, 32, 1 << 40])
     c.write(slots, x, x)
@@ -112,36 +124,35 @@ def test_skipped_and_bad_slots_and_rows_that_are_not_finite(quant):
         assert torch.isnan(k[2, 0]).all() and torch.isnan(v[3, 1]).all()
         assert torch.isfinite(k[2, 1]).all() and torch.isfinite(v[3, 0]).all()
     else:
-        assert torch.equal(k[3].view(torch.int16), x[3].view(torch.int16))
+        assert torch.equal(bits(k[3].contiguous()), bits(x[3]))
     c.write(slots[:0], x[:0], x[:0])
 
 
 def paged(c, q, table, lens, max_len, cap=0.0, dist=None, status=True):
+    """q [n][heads][D]; its rows on the device lie one head further apart.  (o, lse), the call made twice."""
     L = lib.lib()
     n, H, D = q.shape
+    wide = Dev(torch.cat([q, q[:, :1]], 1))
     a = lib.PagedAttn()
     a.n_seqs, a.n_q_heads, a.max_pages, a.max_len = n, H, table.shape[1], max_len
-    a.q, a.q_seq, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
-    t, ln = table.int().cuda(), lens.int().cuda()
-    a.block_table, a.seq_lens = t.data_ptr(), ln.data_ptr()
+    a.q, a.q_seq, a.q_head = wide.ptr, (H + 1) * D, D
+    t, ln = Dev(table.int()), Dev(lens.int())
+    a.block_table, a.seq_lens = t.ptr, ln.ptr
     a.scale, a.cap = 1 / math.sqrt(D), cap
     if dist is not None:
-        d = dist.cuda()
-        a.dist_bias, a.bias_radius = d.data_ptr(), (dist.shape[1] - 1) // 2
-    o = torch.full((n, H, D), float("nan"), dtype=q.dtype, device="cuda")
-    lse = torch.full((n, H), float("nan"), device="cuda")
-    a.o, a.o_seq, a.o_head, a.lse = o.data_ptr(), H * D, D, lse.data_ptr()
+        d = Dev(dist)
+        a.dist_bias, a.bias_radius = d.ptr, (dist.shape[1] - 1) // 2
+    o, lse = full((n, H, D), float("nan"), q.dtype), full((n, H), float("nan"))
+    a.o, a.o_seq, a.o_head, a.lse = o.ptr, H * D, D, lse.ptr
     size = L.vdk_paged_attention_workspace_size(c.d, a)
-    work = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device="cuda")
-    a.work, a.work_bytes, a.status = work.data_ptr(), size, c.status.data_ptr() if status else None
+    work = full((max(size, 1),), 0xff, torch.uint8)
+    a.work, a.work_bytes, a.status = work.ptr, size, c.status.ptr if status else None
     lib.check(L.vdk_paged_attention(c.d, a, None))
-    torch.cuda.synchronize()
-    first = o.clone()
-    o.zero_()
+    first = o.get()
+    o.put(torch.zeros_like(first))
     lib.check(L.vdk_paged_attention(c.d, a, None))
-    torch.cuda.synchronize()
-    assert torch.equal(o.view(torch.int16), first.view(torch.int16))
-    return o, lse
+    assert torch.equal(bits(o.get()), bits(first))
+    return o.get(), lse.get()
 
 
 def streams(lens, page, kv, D, dtype, quant, H, seed=0):
@@ -160,15 +171,10 @@ def streams(lens, page, kv, D, dtype, quant, H, seed=0):
             continue
         j = torch.arange(n)
         slots = table[i, j // page] * page + j % page
-        k, v = (torch.randn(n, kv, D, generator=g).to(c.t).cuda() for _ in range(2))
+        k, v = (torch.randn(n, kv, D, generator=g).to(c.t) for _ in range(2))
         c.write(slots, k, v)
-        if quant:
-            rows.append(tuple((held[slots // page, :, slots % page].view(torch.float8_e4m3fn).float().double()
-                               * s[slots // page, :, slots % page].double()[..., None]).cpu()
-                              for held, s in ((c.k, c.ks), (c.v, c.vs))))
-        else:
-            rows.append((k.double().cpu(), v.double().cpu()))
-    q = (torch.randn(len(lens), H + 1, D, generator=g) * 1.2).to(c.t).cuda()[:, :H]
+        rows.append(c.held(slots))
+    q = (torch.randn(len(lens), H + 1, D, generator=g) * 1.2).to(c.t)[:, :H]
     return c, table, rows, q
 
 
@@ -176,14 +182,14 @@ def expected(rows, q, lens, cap, dist, dtype):
     """o, lse and their bounds: those of attn_ref with the value's scale (one more rounding of P)."""
     o, lse, to, tl = [], [], [], []
     for i, (k, v) in enumerate(rows):
-        out, tol = ref.attend(q[i:i + 1].cpu().double(), k.double(), v.double(), [0, 1], [0, lens[i]], 1 / math.sqrt(q.shape[2]), cap,
+        out, tol = ref.attend(q[i:i + 1].double(), k.double(), v.double(), [0, 1], [0, lens[i]], 1 / math.sqrt(q.shape[2]), cap,
                               dist, False, None)
         u, fl = ref.half_step(dtype), ref.floor16(dtype)
         H, G = q.shape[1], q.shape[1] // k.shape[1]
         P = torch.zeros(q.shape[1], q.shape[2], dtype=torch.float64)
         for h in range(H):
             kk, vv = k[:, h // G].double(), v[:, h // G].double()
-            s, _, _, _ = ref.scores(q[i, h:h + 1].cpu().double(), kk, 1 / math.sqrt(q.shape[2]), cap,
+            s, _, _, _ = ref.scores(q[i, h:h + 1].double(), kk, 1 / math.sqrt(q.shape[2]), cap,
                                     None if dist is None else dist[h].double(),
                                     0 if dist is None else (dist.shape[1] - 1) // 2, lens[i] - 1, torch.tensor([lens[i]]))
             p, _ = ref.softmax(s)
@@ -227,13 +233,12 @@ def test_values_far_from_one_keep_their_precision(scale):
     """f16 rows of very small or large values: a value's scale times p would leave f16."""
     c, table, _, q = streams([300], 32, 2, 64, "f16", True, 4)
     g = torch.Generator().manual_seed(9)
-    k = torch.randn(300, 2, 64, generator=g).half().cuda()
-    v = (torch.randn(300, 2, 64, generator=g) * scale).half().cuda()
+    k = torch.randn(300, 2, 64, generator=g).half()
+    v = (torch.randn(300, 2, 64, generator=g) * scale).half()
     j = torch.arange(300)
     slots = table[0, j // 32] * 32 + j % 32
     c.write(slots, k, v)
-    rows = [tuple((held[slots // 32, :, slots % 32].view(torch.float8_e4m3fn).float().double()
-                   * s[slots // 32, :, slots % 32].double()[..., None]).cpu() for held, s in ((c.k, c.ks), (c.v, c.vs)))]
+    rows = [c.held(slots)]
     o, lse = paged(c, q, table, torch.tensor([300]), 300)
     wo, wl, to, tl = expected(rows, q, [300], 0.0, None, c.t)
     ref.check(o, wo, to, "o")

@@ -1,12 +1,12 @@
 """vdk_relpos_attention, its backward pass and the bias by buckets against their
 formulas in 64 bits (attn_ref.py), elementwise within bounds counted there."""
-import ctypes as C
 import math
 
 import pytest
 import torch
 
 import attn_ref as ref
+from attn_gpu import Dev, Stream, full
 from gpu_util import announce, device_ok
 from vdamd import lib
 
@@ -39,63 +39,52 @@ class Layer:
         self.dist = torch.randn(H, 2 * R + 1, generator=g) if R else None
 
     def up(self):
-        """To the GPU with the strides kept."""
-        def put(x):
-            if x is None:
-                return None
-            base = torch.zeros(x.shape[0], x.stride(0) // x.shape[2] if x.shape[0] else 1, x.shape[2], dtype=x.dtype,
-                               device="cuda")
-            y = base[:, :x.shape[1]]
-            y.copy_(x)
-            return y
-        self.g = {n: put(getattr(self, n)) for n in ("q", "k", "v", "do")}
-        self.g["dist"] = None if self.dist is None else self.dist.cuda()
+        """To the GPU, the strides kept: k and v are halves of one buffer."""
+        n, m, H, D, kv = self.q_at[-1], self.kv_at[-1], self.H, self.D, self.kv
+        wide = torch.zeros(n, H + 1, D, dtype=self.t)
+        wide[:, :H] = self.q
+        self.g = {"q": Dev(wide), "kv": Dev(torch.cat([self.k, self.v], 1)), "do": Dev(self.do),
+                  "dist": None if self.dist is None else Dev(self.dist)}
         a = self.a = lib.RelposAttn()
         a.dtype, a.scale, a.cap = (lib.F16 if self.t == torch.float16 else lib.BF16), self.scale, self.cap
-        for x in ("q", "k", "v"):
-            y = self.g[x]
-            setattr(a, x, y.data_ptr())
-            setattr(a, x + "_tok", y.stride(0))
-            setattr(a, x + "_head", y.stride(1))
+        for x, ptr, tok in (("q", self.g["q"].ptr, (H + 1) * D), ("k", self.g["kv"].ptr, 2 * kv * D),
+                            ("v", self.g["kv"].at(kv * D), 2 * kv * D)):
+            setattr(a, x, ptr)
+            setattr(a, x + "_tok", tok)
+            setattr(a, x + "_head", D)
         if self.R:
-            a.dist_bias, a.bias_radius = self.g["dist"].data_ptr(), self.R
-        n, m, H, D = self.q_at[-1], self.kv_at[-1], self.H, self.D
+            a.dist_bias, a.bias_radius = self.g["dist"].ptr, self.R
         nan = float("nan")
-        self.o = torch.full((n, H, D), nan, dtype=self.t, device="cuda")
-        self.o32 = torch.full((n, H, D), nan, device="cuda")
-        self.lse = torch.full((H, n), nan, device="cuda")
-        a.o, a.o_tok, a.o_head = self.o.data_ptr(), H * D, D
-        a.lse = self.lse.data_ptr()
-        self.plan = lib.AttnPlan(self.q_at, self.kv_at, H, self.kv, D, causal=self.causal, prefix=self.prefix)
+        self.o, self.o32, self.lse = full((n, H, D), nan, self.t), full((n, H, D), nan), full((H, n), nan)
+        a.o, a.o_tok, a.o_head = self.o.ptr, H * D, D
+        a.lse = self.lse.ptr
+        self.plan = lib.AttnPlan(self.q_at, self.kv_at, H, kv, D, causal=self.causal, prefix=self.prefix)
         return self
 
-    def forward(self, train=False):
-        self.a.o_f32 = self.o32.data_ptr() if train else None
-        lib.check(lib.lib().vdk_relpos_attention(self.plan.ptr, self.a, None))
-        torch.cuda.synchronize()
+    def forward(self, train=False, stream=None):
+        self.a.o_f32 = self.o32.ptr if train else None
+        lib.check(lib.lib().vdk_relpos_attention(self.plan.ptr, self.a, stream))
         return {"o": self.o, "lse": self.lse}
 
     def backward(self):
         L, H, D = lib.lib(), self.H, self.D
         n, m = self.q_at[-1], self.kv_at[-1]
         nan = float("nan")
-        self.dq = torch.full((n, H, D), nan, dtype=self.t, device="cuda")
-        self.dk, self.dv = (torch.full((m, self.kv, D), nan, dtype=self.t, device="cuda") for _ in range(2))
-        b = lib.RelposAttnGrad()
-        b.d_o, b.do_tok, b.do_head = self.g["do"].data_ptr(), self.g["do"].stride(0), self.g["do"].stride(1)
-        b.dq, b.dq_tok, b.dq_head = self.dq.data_ptr(), H * D, D
-        b.dk, b.dk_tok, b.dk_head = self.dk.data_ptr(), self.kv * D, D
-        b.dv, b.dv_tok, b.dv_head = self.dv.data_ptr(), self.kv * D, D
+        self.dq = full((n, H, D), nan, self.t)
+        self.dk, self.dv = (full((m, self.kv, D), nan, self.t) for _ in range(2))
+        b = self.b = lib.RelposAttnGrad()
+        b.d_o, b.do_tok, b.do_head = self.g["do"].ptr, H * D, D
+        b.dq, b.dq_tok, b.dq_head = self.dq.ptr, H * D, D
+        b.dk, b.dk_tok, b.dk_head = self.dk.ptr, self.kv * D, D
+        b.dv, b.dv_tok, b.dv_head = self.dv.ptr, self.kv * D, D
         out = {"dq": self.dq, "dk": self.dk, "dv": self.dv}
         if self.R:
-            self.ddist = torch.full((H, 2 * self.R + 1), nan, device="cuda")
-            b.d_dist_bias = self.ddist.data_ptr()
-            out["ddist"] = self.ddist
+            self.ddist = out["ddist"] = full((H, 2 * self.R + 1), nan)
+            b.d_dist_bias = self.ddist.ptr
         size = L.vdk_relpos_attention_backward_workspace_size(self.plan.ptr, self.R)
-        self.work = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device="cuda")
-        b.work, b.work_bytes = self.work.data_ptr(), size
+        self.work = full((max(size, 1),), 0xff, torch.uint8)
+        b.work, b.work_bytes = self.work.ptr, size
         lib.check(L.vdk_relpos_attention_backward(self.plan.ptr, self.a, b, None))
-        torch.cuda.synchronize()
         return out
 
     def reference(self, grad=False):
@@ -143,10 +132,10 @@ def test_forward(case, train):
     want, tol = x.reference()
     got = x.up().forward(train)
     for n in ("o", "lse"):
-        ref.check(got[n], want[n], tol[n], n)
+        ref.check(got[n].get(), want[n], tol[n], n)
     if train:
         u = ref.half_step(x.t)
-        ref.check(x.o32, want["o"], tol["o"] - u * want["o"].abs(), "o_f32")
+        ref.check(x.o32.get(), want["o"], tol["o"] - u * want["o"].abs(), "o_f32")
 
 
 GRAD = [
@@ -178,12 +167,11 @@ def test_backward(case):
     x = Layer(**case)
     want, tol = x.reference(grad=True)
     x.up().forward(True)
-    got = x.backward()
+    got = {n: y.get() for n, y in x.backward().items()}
     for n, y in got.items():
         ref.check(y, want[n], tol[n], n)
-    again = {n: y.clone() for n, y in got.items()}
     for n, y in x.backward().items():
-        assert torch.equal(y, again[n]), f"{n}: another call, other bits"
+        assert torch.equal(y.get(), got[n]), f"{n}: another call, other bits"
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -197,14 +185,14 @@ def test_gradients_of_very_small_and_uneven_output_gradients(dtype):
     want, tol = x.reference(grad=True)
     x.up().forward(True)
     for n, y in x.backward().items():
-        ref.check(y, want[n], tol[n], n)
+        ref.check(y.get(), want[n], tol[n], n)
 
 
 def test_gradients_against_differences():
     """d loss / d q, k, v, bias along random directions against central differences of the formulas' loss."""
     x = Layer([50, 33], 4, 2, 64, "f16", R=12, cap=25.0, causal=True, prefix=[4, 0])
     x.up().forward(True)
-    got = {n: y.double().cpu() for n, y in x.backward().items()}
+    got = {n: y.get().double() for n, y in x.backward().items()}
     g = torch.Generator().manual_seed(5)
 
     def loss(q, k, v, dist):
@@ -233,12 +221,12 @@ def test_biases_of_minus_infinity_and_of_the_lowest_value():
     for z in (x, y):
         want, tol = z.reference(grad=z is x)
         got = z.up().forward(True)
-        ref.check(got["o"], want["o"], tol["o"], "o")
-        ref.check(got["lse"], want["lse"], tol["lse"], "lse")
-    assert (x.o[:, 1] == 0).all() and torch.isneginf(x.lse[1]).all()
+        ref.check(got["o"].get(), want["o"], tol["o"], "o")
+        ref.check(got["lse"].get(), want["lse"], tol["lse"], "lse")
+    assert (x.o.get()[:, 1] == 0).all() and torch.isneginf(x.lse.get()[1]).all()
     want, tol = x.reference(grad=True)
     for n, v in x.backward().items():
-        ref.check(v, want[n], tol[n], n)
+        ref.check(v.get(), want[n], tol[n], n)
 
 
 def test_clips_do_not_reach_each_other():
@@ -250,7 +238,7 @@ def test_clips_do_not_reach_each_other():
     got = dict(x.backward(), o=x.o)
     keep = [i for i in range(203) if not 100 <= i < 133]
     for n in ("o", "dq", "dk", "dv"):
-        ref.check(got[n][keep], want[n][keep], tol[n][keep], n)
+        ref.check(got[n].get()[keep], want[n][keep], tol[n][keep], n)
 
 
 @pytest.mark.parametrize("cap", [2.0, 5.0])
@@ -262,47 +250,38 @@ def test_scores_far_past_the_cap(cap):
     want, tol = x.reference(grad=True)
     got = x.up().forward(True)
     for n, y in dict(got, **x.backward()).items():
-        ref.check(y, want[n], tol[n], n)
+        ref.check(y.get(), want[n], tol[n], n)
 
 
 def test_same_results_on_another_stream_and_in_a_graph():
     x = Layer([149, 60], 4, 2, 64, "f16", R=128, cap=30.0).up()
-    x.forward(True)
-    first = dict(x.forward(True), **x.backward())
-    first = {n: y.clone() for n, y in first.items()}
-    s = torch.cuda.Stream()
-    L = lib.lib()
-    b = lib.RelposAttnGrad()
-    n, m, H, D = x.q_at[-1], x.kv_at[-1], x.H, x.D
-    b.d_o, b.do_tok, b.do_head = x.g["do"].data_ptr(), H * D, D
-    b.dq, b.dq_tok, b.dq_head = x.dq.data_ptr(), H * D, D
-    b.dk, b.dk_tok, b.dk_head = x.dk.data_ptr(), x.kv * D, D
-    b.dv, b.dv_tok, b.dv_head = x.dv.data_ptr(), x.kv * D, D
-    b.d_dist_bias, b.work, b.work_bytes = x.ddist.data_ptr(), x.work.data_ptr(), x.work.numel()
-    outs = {"o": x.o, "lse": x.lse, "dq": x.dq, "dk": x.dk, "dv": x.dv, "ddist": x.ddist}
+    outs = dict(x.forward(True), **x.backward())
+    first = {n: y.get() for n, y in outs.items()}
+    L, s = lib.lib(), Stream()
 
-    def call():
-        p = torch.cuda.current_stream().cuda_stream
-        lib.check(L.vdk_relpos_attention(x.plan.ptr, x.a, p))
-        lib.check(L.vdk_relpos_attention_backward(x.plan.ptr, x.a, b, p))
-    with torch.cuda.stream(s):
-        for y in outs.values():
-            y.zero_()
-        call()
-    torch.cuda.synchronize()
-    for n_, y in outs.items():
-        assert torch.equal(y, first[n_]), n_
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        call()
+    def call(stream):
+        lib.check(L.vdk_relpos_attention(x.plan.ptr, x.a, stream))
+        lib.check(L.vdk_relpos_attention_backward(x.plan.ptr, x.a, x.b, stream))
+
+    def same():
+        for n, y in outs.items():
+            assert torch.equal(y.get(), first[n]), n
+
+    def clear():
+        for n, y in outs.items():
+            y.put(torch.zeros_like(first[n]))
+    clear()
+    call(s.ptr)
+    s.synchronize()
+    same()
+    launch = s.capture(call)
     for _ in range(3):
-        for y in outs.values():
-            y.zero_()
-        graph.replay()
-        torch.cuda.synchronize()
-        for n_, y in outs.items():
-            assert torch.equal(y, first[n_]), n_
-        x.forward(True)
+        clear()
+        launch()
+        s.synchronize()
+        same()
+        x.forward(True)                            # the program's own work between the replays
+        lib.check(L.vdk_synchronize())
 
 
 BUCKETS = [(32, 1, 128, 128), (320, 1, 800, 800), (32, 0, 128, 200), (5, 0, 7, 30), (4, 1, 3, 1), (1024, 1, 4000, 4096)]
@@ -312,12 +291,11 @@ BUCKETS = [(32, 1, 128, 128), (320, 1, 800, 800), (32, 0, 128, 200), (5, 0, 7, 3
 def test_bias_by_buckets_and_its_gradient(nb, both, far, R):
     H, L = 5, lib.lib()
     g = torch.Generator().manual_seed(nb)
-    table, grad = torch.randn(nb, H, generator=g).cuda(), torch.randn(H, 2 * R + 1, generator=g).cuda()
-    dist, dtable = torch.empty(H, 2 * R + 1, device="cuda"), torch.full((nb, H), float("nan"), device="cuda")
-    lib.check(L.vdk_rel_bias_expand(table.data_ptr(), nb, H, both, far, R, dist.data_ptr(), None))
-    lib.check(L.vdk_rel_bias_reduce(grad.data_ptr(), nb, H, both, far, R, dtable.data_ptr(), None))
-    torch.cuda.synchronize()
+    table, grad = torch.randn(nb, H, generator=g), torch.randn(H, 2 * R + 1, generator=g)
+    d_table, d_grad, dist, dtable = Dev(table), Dev(grad), full((H, 2 * R + 1), 0.0), full((nb, H), float("nan"))
+    lib.check(L.vdk_rel_bias_expand(d_table.ptr, nb, H, both, far, R, dist.ptr, None))
+    lib.check(L.vdk_rel_bias_reduce(d_grad.ptr, nb, H, both, far, R, dtable.ptr, None))
     at = torch.tensor([ref.bucket(r, nb, both, far) for r in range(-R, R + 1)])
-    assert torch.equal(dist.cpu(), table.cpu()[at].t())
-    want = torch.zeros(nb, H, dtype=torch.float64).index_add_(0, at, grad.cpu().double().t())
-    ref.check(dtable, want, ref.F32 * want.abs() + 1e-12, "table gradient")   # 64-bit sums, one rounding
+    assert torch.equal(dist.get(), table[at].t())
+    want = torch.zeros(nb, H, dtype=torch.float64).index_add_(0, at, grad.double().t())
+    ref.check(dtable.get(), want, ref.F32 * want.abs() + 1e-12, "table gradient")   # 64-bit sums, one rounding

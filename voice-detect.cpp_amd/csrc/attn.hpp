@@ -2,6 +2,7 @@
 // swizzled LDS tiles, the score map, and a packed layout's plan.
 #pragma once
 
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <vector>
@@ -301,6 +302,25 @@ struct AttnTile {
     int b32;                // blocks of 32 queries before the clip's
     int row, pad;
 };
+
+// require() whose message is put together only where it is thrown.
+#define VDK_NEED(ok, ...)                          \
+    do {                                           \
+        if (!(ok)) throw ::vdk::Error(__VA_ARGS__); \
+    } while (0)
+
+// Launches of more than 64 KB of LDS have to be allowed: once a kernel, device and size not seen before.
+template <auto KERN>
+void allow_lds(size_t bytes) {
+    static std::atomic<size_t> allowed[16];
+    if (bytes <= 65536) return;
+    int dev = 0;
+    VDK_HIP(hipGetDevice(&dev));
+    std::atomic<size_t>& most = allowed[dev & 15];
+    if (dev < 16 && most.load(std::memory_order_relaxed) >= bytes) return;
+    VDK_HIP(hipFuncSetAttribute((const void*)KERN, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    most.store(bytes, std::memory_order_relaxed);   // (a smaller size stored by another thread only costs a call)
+}
 
 // Argument checks shared by the forward and the backward call.
 void check_rows(const void* p, long long tok, long long head, int dim, const char* name);

@@ -497,24 +497,26 @@ __global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs a) {
                                     : -FLT_MAX;
 }
 
-void check_cache(const vdk_kv_cache* c, const std::string& w) {
-    require(c, w + ": NULL cache");
-    require(c->dtype == VDK_F16 || c->dtype == VDK_BF16, w + ": dtype must be VDK_F16 or VDK_BF16");
-    require(c->format == VDK_KV_16 || c->format == VDK_KV_E4M3, w + ": format must be VDK_KV_16 or VDK_KV_E4M3");
-    require(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
-            w + ": page_size must be 16, 32, 64 or 128");
-    require(c->head_dim == 64 || c->head_dim == 128, w + ": head_dim must be 64 or 128");
-    require(c->n_pages > 0 && c->n_kv_heads > 0 && c->n_kv_heads <= 1024, w + ": empty cache or too many heads");
-    require(c->k && c->v && (c->format == VDK_KV_16 || (c->k_scale && c->v_scale)), w + ": NULL cache pointer");
-    require((uintptr_t)c->k % 16 == 0 && (uintptr_t)c->v % 16 == 0 && (uintptr_t)c->k_scale % 16 == 0 &&
+void check_cache(const vdk_kv_cache* c, const char* what) {
+    auto w = [&] { return std::string(what); };
+    VDK_NEED(c, w() + ": NULL cache");
+    VDK_NEED(c->dtype == VDK_F16 || c->dtype == VDK_BF16, w() + ": dtype must be VDK_F16 or VDK_BF16");
+    VDK_NEED(c->format == VDK_KV_16 || c->format == VDK_KV_E4M3, w() + ": format must be VDK_KV_16 or VDK_KV_E4M3");
+    VDK_NEED(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
+            w() + ": page_size must be 16, 32, 64 or 128");
+    VDK_NEED(c->head_dim == 64 || c->head_dim == 128, w() + ": head_dim must be 64 or 128");
+    VDK_NEED(c->n_pages > 0 && c->n_kv_heads > 0 && c->n_kv_heads <= 1024, w() + ": empty cache or too many heads");
+    VDK_NEED(c->k && c->v && (c->format == VDK_KV_16 || (c->k_scale && c->v_scale)), w() + ": NULL cache pointer");
+    VDK_NEED((uintptr_t)c->k % 16 == 0 && (uintptr_t)c->v % 16 == 0 && (uintptr_t)c->k_scale % 16 == 0 &&
                 (uintptr_t)c->v_scale % 16 == 0,
-            w + ": cache pointers must be 16-byte aligned");
+            w() + ": cache pointers must be 16-byte aligned");
 }
 
-void check_strided(const void* p, long long a, long long b, const std::string& w) {
-    require(p, w + " is NULL");
-    require((uintptr_t)p % 16 == 0 && a % 8 == 0 && b % 8 == 0 && a >= 0 && b >= 0,
-            w + ": 16-byte aligned pointer and strides of multiples of 8, please");
+void check_strided(const void* p, long long a, long long b, const char* what, const char* name) {
+    auto w = [&] { return std::string(what) + ": " + name; };
+    VDK_NEED(p, w() + " is NULL");
+    VDK_NEED((uintptr_t)p % 16 == 0 && a % 8 == 0 && b % 8 == 0 && a >= 0 && b >= 0,
+            w() + ": 16-byte aligned pointer and strides of multiples of 8, please");
 }
 
 int shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
@@ -523,15 +525,15 @@ template <bool WRITE>
 int cache_rows(const vdk_kv_cache* c, const long long* slots, long long n, void* k, long long k_tok, long long k_head,
                void* v, long long v_tok, long long v_head, int* status, void* stream, const char* what) {
     return guarded([&] {
-        const std::string w(what);
-        check_cache(c, w);
-        require(n >= 0, w + ": negative number of tokens");
+        auto w = [&] { return std::string(what); };
+        check_cache(c, what);
+        VDK_NEED(n >= 0, w() + ": negative number of tokens");
         if (n == 0) return;
-        require(slots && (uintptr_t)slots % 8 == 0 && (uintptr_t)status % 4 == 0, w + ": NULL or misaligned slots");
-        check_strided(k, k_tok, k_head, w + ": k");
-        check_strided(v, v_tok, v_head, w + ": v");
+        VDK_NEED(slots && (uintptr_t)slots % 8 == 0 && (uintptr_t)status % 4 == 0, w() + ": NULL or misaligned slots");
+        check_strided(k, k_tok, k_head, what, "k");
+        check_strided(v, v_tok, v_head, what, "v");
         const long long threads = n * c->n_kv_heads * (c->head_dim / 16);
-        require(n <= (1ll << 40) / c->n_kv_heads && threads <= (1ll << 38), w + ": too many tokens for one launch");
+        VDK_NEED(n <= (1ll << 40) / c->n_kv_heads && threads <= (1ll << 38), w() + ": too many tokens for one launch");
         RowArgs a{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, slots, n,
                   (long long)c->n_pages * c->page_size, c->n_kv_heads, c->page_size, shift_of(c->page_size), k, v,
                   k_tok, k_head, v_tok, v_head, status};
@@ -564,22 +566,21 @@ Cut cut_of(const vdk_kv_cache* c, const vdk_paged_attn* a) {
 }
 
 void check_paged(const vdk_kv_cache* c, const vdk_paged_attn* a) {
-    const std::string w("paged_attention");
-    check_cache(c, w);
-    require(a, w + ": NULL description");
-    require(a->n_seqs >= 0 && a->max_pages >= 0 && a->max_len >= 0, w + ": negative size");
-    require(a->n_q_heads > 0 && a->n_q_heads % c->n_kv_heads == 0 && a->n_q_heads <= 1024,
-            w + ": n_q_heads must be a multiple of n_kv_heads, at most 1024");
-    require(a->max_len <= (long long)a->max_pages * c->page_size, w + ": max_len exceeds the block table");
-    require(a->max_len <= (1 << 30), w + ": max_len must be 2^30 at most");
+    auto w = [] { return std::string("paged_attention"); };
+    check_cache(c, "paged_attention");
+    VDK_NEED(a, w() + ": NULL description");
+    VDK_NEED(a->n_seqs >= 0 && a->max_pages >= 0 && a->max_len >= 0, w() + ": negative size");
+    VDK_NEED(a->n_q_heads > 0 && a->n_q_heads % c->n_kv_heads == 0 && a->n_q_heads <= 1024,
+            w() + ": n_q_heads must be a multiple of n_kv_heads, at most 1024");
+    VDK_NEED(a->max_len <= (long long)a->max_pages * c->page_size, w() + ": max_len exceeds the block table");
+    VDK_NEED(a->max_len <= (1 << 30), w() + ": max_len must be 2^30 at most");
 }
 
 template <class T, int D, bool QUANT, bool CAP, int kWaves>
 void launch_parts(const PagedArgs& a, int n, hipStream_t s) {
-    auto kern = paged_attn_kernel<T, D, QUANT, CAP, kWaves>;
+    constexpr auto kern = paged_attn_kernel<T, D, QUANT, CAP, kWaves>;
     const int lds = PagedShape<T, D, QUANT, kWaves>::kLds + 4 * (a.chunk >> a.page_shift) + 4 * std::min(a.group, 16) * a.span;
-    if (lds > 65536)
-        VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    allow_lds<kern>(lds);
     hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * kWaves), lds, s, a);
     VDK_HIP(hipGetLastError());
 }
@@ -638,29 +639,29 @@ extern "C" size_t vdk_paged_attention_workspace_size(const vdk_kv_cache* c, cons
 
 extern "C" int vdk_paged_attention(const vdk_kv_cache* c, const vdk_paged_attn* a, void* stream) {
     return guarded([&] {
-        const std::string w("paged_attention");
+        auto w = [] { return std::string("paged_attention"); };
         check_paged(c, a);
-        require(std::isfinite(a->scale) && a->scale > 0.0f, w + ": scale must be positive and finite");
-        require(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
-                w + ": cap must be 0 or 1e-3 .. 1e6");
-        require(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= 4096), w + ": bias_radius must be 1 .. 4096");
+        VDK_NEED(std::isfinite(a->scale) && a->scale > 0.0f, w() + ": scale must be positive and finite");
+        VDK_NEED(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
+                w() + ": cap must be 0 or 1e-3 .. 1e6");
+        VDK_NEED(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= 4096), w() + ": bias_radius must be 1 .. 4096");
         if (a->n_seqs == 0) return;
-        require(a->seq_lens && (a->block_table || a->max_len == 0), w + ": NULL table or lengths");
-        require((uintptr_t)a->seq_lens % 4 == 0 && (uintptr_t)a->block_table % 4 == 0 && (uintptr_t)a->dist_bias % 4 == 0 &&
+        VDK_NEED(a->seq_lens && (a->block_table || a->max_len == 0), w() + ": NULL table or lengths");
+        VDK_NEED((uintptr_t)a->seq_lens % 4 == 0 && (uintptr_t)a->block_table % 4 == 0 && (uintptr_t)a->dist_bias % 4 == 0 &&
                     (uintptr_t)a->lse % 4 == 0 && (uintptr_t)a->status % 4 == 0,
-                w + ": misaligned pointer");
-        check_strided(a->q, a->q_seq, a->q_head, w + ": q");
-        check_strided(a->o, a->o_seq, a->o_head, w + ": o");
+                w() + ": misaligned pointer");
+        check_strided(a->q, a->q_seq, a->q_head, "paged_attention", "q");
+        check_strided(a->o, a->o_seq, a->o_head, "paged_attention", "o");
         const Cut cut = cut_of(c, a);
         const int group = a->n_q_heads / c->n_kv_heads, parts = cdiv(group, 16);
         if (cut.splits > 1) {
             const size_t need = vdk_paged_attention_workspace_size(c, a);
-            require(a->work && a->work_bytes >= need && (uintptr_t)a->work % 16 == 0,
-                    w + ": workspace missing, misaligned or smaller than vdk_paged_attention_workspace_size");
+            VDK_NEED(a->work && a->work_bytes >= need && (uintptr_t)a->work % 16 == 0,
+                    w() + ": workspace missing, misaligned or smaller than vdk_paged_attention_workspace_size");
         }
-        require((long long)a->n_seqs * c->n_kv_heads * parts * cut.splits < (1ll << 31) &&
+        VDK_NEED((long long)a->n_seqs * c->n_kv_heads * parts * cut.splits < (1ll << 31) &&
                     (long long)a->n_seqs * a->n_q_heads < (1ll << 31),
-                w + ": too many streams for one launch");
+                w() + ": too many streams for one launch");
         PagedArgs p{static_cast<const uint8_t*>(c->k), static_cast<const uint8_t*>(c->v), c->k_scale, c->v_scale,
                     c->n_pages, shift_of(c->page_size), c->n_kv_heads, a->q, a->q_seq, a->q_head, a->block_table,
                     a->seq_lens, a->max_pages, a->max_len, a->n_q_heads, group, parts, cut.splits, cut.chunk,

@@ -77,7 +77,10 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
     float far_l = 0.0f, far_r = 0.0f;
     if (R) {
         const float* b = a.bias + (long long)h * (2 * R + 1);
-        for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+        // (the distances that the tile reaches)
+        const int i0 = max(R + kTabPad - 32 - (past + c.row + kRows), 0);
+        const int i1 = min(R + kTabPad + 96 + kend - (past + c.row), 2 * R + 1 + 2 * kTabPad);
+        for (int i = i0 + threadIdx.x; i < i1; i += 64 * NW)
             tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
         far_l = bias2_of(b[0]);
         far_r = bias2_of(b[2 * R]);
@@ -337,21 +340,20 @@ __global__ __launch_bounds__(64) void rel_bias_reduce_kernel(const float* __rest
 
 void check_buckets(const void* src, const void* dst, int n_buckets, int n_heads, int bidirectional, int max_distance,
                    int R, const char* what) {
-    const std::string w(what);
-    require(src && dst, w + ": NULL device pointer");
-    require(n_heads > 0 && n_heads <= 65535, w + ": n_heads must be 1 .. 65535");
-    require(n_buckets >= 4 && n_buckets <= (bidirectional ? 2 : 1) * kMaxHalf && (!bidirectional || n_buckets % 2 == 0),
-            w + ": n_buckets must be 4 .. 512 (bidirectional: even, 4 .. 1024)");
-    require(max_distance > (bidirectional ? n_buckets / 2 : n_buckets) / 2,
-            w + ": max_distance must exceed the buckets of one distance each");
-    require(R >= 1 && R <= kMaxRadius, w + ": bias_radius must be 1 .. 4096");
+    auto w = [&] { return std::string(what); };
+    VDK_NEED(src && dst, w() + ": NULL device pointer");
+    VDK_NEED(n_heads > 0 && n_heads <= 65535, w() + ": n_heads must be 1 .. 65535");
+    VDK_NEED(n_buckets >= 4 && n_buckets <= (bidirectional ? 2 : 1) * kMaxHalf && (!bidirectional || n_buckets % 2 == 0),
+            w() + ": n_buckets must be 4 .. 512 (bidirectional: even, 4 .. 1024)");
+    VDK_NEED(max_distance > (bidirectional ? n_buckets / 2 : n_buckets) / 2,
+            w() + ": max_distance must exceed the buckets of one distance each");
+    VDK_NEED(R >= 1 && R <= kMaxRadius, w() + ": bias_radius must be 1 .. 4096");
 }
 
 template <class T, int D, bool CAP, bool SPLIT, bool NARROW>
 void launch_tiles(const vdk_attn_plan* p, FwdArgs a, size_t lds, hipStream_t s) {
-    auto kern = relpos_fwd_kernel<T, D, CAP, SPLIT, NARROW>;
-    if (lds > 65536)
-        VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    constexpr auto kern = relpos_fwd_kernel<T, D, CAP, SPLIT, NARROW>;
+    allow_lds<kern>(lds);
     a.tiles = NARROW ? p->d_b32 : p->d_q128;
     a.n_tiles = NARROW ? p->n_b32 : p->n_q128;
     hipLaunchKernelGGL(kern, dim3((unsigned)a.n_tiles * a.n_heads), dim3(256), lds, s, a);
@@ -379,22 +381,21 @@ void launch_fwd_t(const vdk_attn_plan* p, const FwdArgs& a, bool cap, hipStream_
 }  // namespace
 
 void check_rows(const void* p, long long tok, long long head, int dim, const char* name) {
-    const std::string w(name);
-    require(p, "relpos_attention: " + w + " is NULL");
-    require((uintptr_t)p % 16 == 0, "relpos_attention: " + w + " must be 16-byte aligned");
-    require(tok % 8 == 0 && head % 8 == 0 && tok >= dim && tok <= (1 << 22) && head >= 0 && head <= (1ll << 40),
-            "relpos_attention: strides of " + w + " must be multiples of 8, between tokens head_dim .. 2^22");
+    VDK_NEED(p, "relpos_attention: " + std::string(name) + " is NULL");
+    VDK_NEED((uintptr_t)p % 16 == 0, "relpos_attention: " + std::string(name) + " must be 16-byte aligned");
+    VDK_NEED(tok % 8 == 0 && head % 8 == 0 && tok >= dim && tok <= (1 << 22) && head >= 0 && head <= (1ll << 40),
+            "relpos_attention: strides of " + std::string(name) + " must be multiples of 8, between tokens head_dim .. 2^22");
 }
 
 void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a) {
-    require(p && a, "relpos_attention: NULL plan or description");
-    require(a->dtype == VDK_F16 || a->dtype == VDK_BF16, "relpos_attention: dtype must be VDK_F16 or VDK_BF16");
-    require(std::isfinite(a->scale) && a->scale > 0.0f, "relpos_attention: scale must be positive and finite");
-    require(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
+    VDK_NEED(p && a, "relpos_attention: NULL plan or description");
+    VDK_NEED(a->dtype == VDK_F16 || a->dtype == VDK_BF16, "relpos_attention: dtype must be VDK_F16 or VDK_BF16");
+    VDK_NEED(std::isfinite(a->scale) && a->scale > 0.0f, "relpos_attention: scale must be positive and finite");
+    VDK_NEED(std::isfinite(a->cap) && (a->cap == 0.0f || (a->cap >= 1e-3f && a->cap <= 1e6f)),
             "relpos_attention: cap must be 0 or 1e-3 .. 1e6");
-    require(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= kMaxRadius),
+    VDK_NEED(!a->dist_bias || (a->bias_radius >= 1 && a->bias_radius <= kMaxRadius),
             "relpos_attention: bias_radius must be 1 .. 4096");
-    require((uintptr_t)a->dist_bias % 4 == 0 && (uintptr_t)a->lse % 4 == 0 && (uintptr_t)a->o_f32 % 16 == 0,
+    VDK_NEED((uintptr_t)a->dist_bias % 4 == 0 && (uintptr_t)a->lse % 4 == 0 && (uintptr_t)a->o_f32 % 16 == 0,
             "relpos_attention: misaligned pointer");
     if (p->total_q == 0) return;
     check_rows(a->q, a->q_tok, a->q_head, p->dim, "q");
@@ -403,7 +404,7 @@ void check_relpos(const vdk_attn_plan* p, const vdk_relpos_attn* a) {
         check_rows(a->k, a->k_tok, a->k_head, p->dim, "k");
         check_rows(a->v, a->v_tok, a->v_head, p->dim, "v");
     }
-    require(p->device, "relpos_attention: the plan was made without a GPU");
+    VDK_NEED(p->device, "relpos_attention: the plan was made without a GPU");
 }
 
 }  // namespace vdk
@@ -414,14 +415,14 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
                                     int n_kv_heads, int head_dim, int causal, const long long* prefix,
                                     vdk_attn_plan** plan) {
     return guarded([&] {
-        require(plan, "attn_plan: NULL result pointer");
+        VDK_NEED(plan, "attn_plan: NULL result pointer");
         *plan = nullptr;
-        require(n_clips >= 0 && q_offsets && kv_offsets, "attn_plan: NULL offsets or a negative number of clips");
-        require(head_dim == 64 || head_dim == 128, "attn_plan: head_dim must be 64 or 128");
-        require(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 1024,
+        VDK_NEED(n_clips >= 0 && q_offsets && kv_offsets, "attn_plan: NULL offsets or a negative number of clips");
+        VDK_NEED(head_dim == 64 || head_dim == 128, "attn_plan: head_dim must be 64 or 128");
+        VDK_NEED(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 1024,
                 "attn_plan: n_heads must be a multiple of n_kv_heads, at most 1024");
-        require(causal || !prefix, "attn_plan: a prefix needs causal");
-        require(q_offsets[0] == 0 && kv_offsets[0] == 0, "attn_plan: offsets must start at 0");
+        VDK_NEED(causal || !prefix, "attn_plan: a prefix needs causal");
+        VDK_NEED(q_offsets[0] == 0 && kv_offsets[0] == 0, "attn_plan: offsets must start at 0");
         vdk_attn_plan p{};
         p.n_clips = n_clips;
         p.n_heads = n_heads;
@@ -433,10 +434,10 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         int b32 = 0;
         for (int c = 0; c < n_clips; ++c) {
             const long long nq = q_offsets[c + 1] - q_offsets[c], nk = kv_offsets[c + 1] - kv_offsets[c];
-            require(nq >= 0 && nk >= 0 && q_offsets[c] >= 0 && kv_offsets[c] >= 0, "attn_plan: offsets must not fall");
-            require(nq <= (1 << 30) && nk <= (1 << 30), "attn_plan: a clip may hold 2^30 frames at most");
+            VDK_NEED(nq >= 0 && nk >= 0 && q_offsets[c] >= 0 && kv_offsets[c] >= 0, "attn_plan: offsets must not fall");
+            VDK_NEED(nq <= (1 << 30) && nk <= (1 << 30), "attn_plan: a clip may hold 2^30 frames at most");
             const long long pre = prefix ? prefix[c] : 0;
-            require(pre >= 0 && pre <= nk, "attn_plan: a prefix must be 0 .. the clip's keys");
+            VDK_NEED(pre >= 0 && pre <= nk, "attn_plan: a prefix must be 0 .. the clip's keys");
             AttnTile t{q_offsets[c], kv_offsets[c], (int)nq, (int)nk, (int)pre, b32, 0, 0};
             auto at = [&](long long row) {
                 t.row = (int)row;
@@ -448,7 +449,7 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
                 q128.push_back({seen(std::min(q + 128, nq) - 1), at(q)});
             for (long long q = 0; q < nq; q += 32) lists.push_back(at(q));
             b32 += cdiv(nq, 32);
-            require((long long)b32 * n_heads < (1 << 30) && k32.size() * n_heads < (1u << 30),
+            VDK_NEED((long long)b32 * n_heads < (1 << 30) && k32.size() * n_heads < (1u << 30),
                     "attn_plan: too many tiles for one launch");
             for (long long k = 0; k < nk; k += 32) k32.push_back(at(k));
             for (long long k = 0; k < nk; k += 128) {
@@ -458,7 +459,7 @@ extern "C" int vdk_attn_plan_create(int n_clips, const long long* q_offsets, con
         }
         p.total_q = n_clips ? q_offsets[n_clips] : 0;
         p.total_kv = n_clips ? kv_offsets[n_clips] : 0;
-        require(p.total_q <= (1ll << 36) && p.total_kv <= (1ll << 36), "attn_plan: too many frames");
+        VDK_NEED(p.total_q <= (1ll << 36) && p.total_kv <= (1ll << 36), "attn_plan: too many frames");
         for (auto* l : {&q128, &k128}) {
             std::stable_sort(l->begin(), l->end(), [](const auto& x, const auto& y) { return x.first > y.first; });
             for (const auto& t : *l) lists.push_back(t.second);

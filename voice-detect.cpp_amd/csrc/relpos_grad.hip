@@ -165,7 +165,9 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     float far_l = 0.0f, far_r = 0.0f;
     if constexpr (BIAS) {
         const float* b = a.bias + (long long)h * (2 * R + 1);
-        for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+        const int i0 = max(R + kTabPad - 32 - (past + c.row + (NARROW ? 32 : 128)), 0);
+        const int i1 = min(R + kTabPad + 96 + kend - (past + c.row), 2 * R + 1 + 2 * kTabPad);
+        for (int i = i0 + threadIdx.x; i < i1; i += 64 * NW)   // (the distances that the tile reaches)
             tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
         far_l = bias2_of(b[0]);
         far_r = bias2_of(b[2 * R]);
@@ -407,7 +409,9 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
             if (it % per_head == 0) {   // another head's bias
                 lds_barrier();
                 const float* b = a.bias + (long long)h * (2 * R + 1);
-                for (int i = threadIdx.x; i < 2 * R + 1 + 2 * kTabPad; i += 64 * NW)
+                const int i0 = max(R + kTabPad - 160 + c.row - (past + c.nq), 0);
+                const int i1 = min(R + kTabPad + 160 + c.row - (past + q_first), 2 * R + 1 + 2 * kTabPad);
+                for (int i = i0 + threadIdx.x; i < i1; i += 64 * NW)   // (the distances that the tile reaches)
                     tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
                 far_l = bias2_of(b[0]);
                 far_r = bias2_of(b[2 * R]);
@@ -642,9 +646,9 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, const GradCut& cut, hipStre
     const long long n_dkv = (long long)a.n_k * a.n_kv * a.head_parts, n_dkv8 = (n_dkv + 7) / 8 * 8;
     const long long n = n_dkv8 + (long long)a.n_q * a.n_heads;
     if (n > 0) {
+        cut.narrow ? allow_lds<relpos_grad_kernel<T, D, CAP, BIAS, true>>(cut.lds)
+                   : allow_lds<relpos_grad_kernel<T, D, CAP, BIAS, false>>(cut.lds);
         auto kern = cut.narrow ? relpos_grad_kernel<T, D, CAP, BIAS, true> : relpos_grad_kernel<T, D, CAP, BIAS, false>;
-        if (cut.lds > 65536)
-            VDK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, cut.lds));
         hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), cut.lds, s, a, (int)n_dkv, (int)n_dkv8);
         VDK_HIP(hipGetLastError());
         if (a.head_parts > 1) {
@@ -673,8 +677,8 @@ using namespace vdk;
 extern "C" size_t vdk_relpos_attention_backward_workspace_size(const vdk_attn_plan* p, int bias_radius) {
     size_t n = 0;
     if (guarded([&] {
-            require(p, "relpos_attention_backward: NULL plan");
-            require(bias_radius >= 0 && bias_radius <= 4096, "relpos_attention_backward: bias_radius must be 0 .. 4096");
+            VDK_NEED(p, "relpos_attention_backward: NULL plan");
+            VDK_NEED(bias_radius >= 0 && bias_radius <= 4096, "relpos_attention_backward: bias_radius must be 0 .. 4096");
             const GradCut cut = cut_of(p, bias_radius);
             n = cut.head_parts > 1 ? (size_t)cut.head_parts * 2 * p->total_kv * p->n_kv * p->dim * 4 : 0;
             n += up16((size_t)p->n_heads * p->total_q * 4) + up16((size_t)p->n_heads * p->n_b32 * 4) +
@@ -689,22 +693,22 @@ extern "C" int vdk_relpos_attention_backward(const vdk_attn_plan* p, const vdk_r
                                              const vdk_relpos_attn_grad* g, void* stream) {
     return guarded([&] {
         check_relpos(p, a);
-        require(g, "relpos_attention_backward: NULL description");
-        require(!g->d_dist_bias || a->dist_bias, "relpos_attention_backward: d_dist_bias without a bias");
-        require((uintptr_t)g->d_dist_bias % 4 == 0, "relpos_attention_backward: misaligned pointer");
+        VDK_NEED(g, "relpos_attention_backward: NULL description");
+        VDK_NEED(!g->d_dist_bias || a->dist_bias, "relpos_attention_backward: d_dist_bias without a bias");
+        VDK_NEED((uintptr_t)g->d_dist_bias % 4 == 0, "relpos_attention_backward: misaligned pointer");
         const int R = a->dist_bias ? a->bias_radius : 0;
         if (p->total_q > 0) {
-            require(a->o_f32 && a->lse, "relpos_attention_backward: o_f32 and lse of the forward call are missing");
+            VDK_NEED(a->o_f32 && a->lse, "relpos_attention_backward: o_f32 and lse of the forward call are missing");
             check_rows(g->d_o, g->do_tok, g->do_head, p->dim, "d_o");
             check_rows(g->dq, g->dq_tok, g->dq_head, p->dim, "dq");
         }
         if (p->total_kv > 0) {
             check_rows(g->dk, g->dk_tok, g->dk_head, p->dim, "dk");
             check_rows(g->dv, g->dv_tok, g->dv_head, p->dim, "dv");
-            require(p->device, "relpos_attention: the plan was made without a GPU");
+            VDK_NEED(p->device, "relpos_attention: the plan was made without a GPU");
         }
         const size_t need = vdk_relpos_attention_backward_workspace_size(p, R);
-        require(need == 0 || (g->work && g->work_bytes >= need && (uintptr_t)g->work % 16 == 0),
+        VDK_NEED(need == 0 || (g->work && g->work_bytes >= need && (uintptr_t)g->work % 16 == 0),
                 "relpos_attention_backward: workspace missing, misaligned or too small");
         GradArgs f{};
         f.q = a->q; f.k = a->k; f.v = a->v; f.d_o = g->d_o;
