@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
     constexpr int NW = 4, kRows = NARROW ? 32 : 128, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
-    const int2 ht = head_tile(blockIdx.x, a.n_tiles, a.n_heads);
+    const int2 ht = head_tile(blockIdx.x, a.n_tiles, a.n_heads, a.causal);
     const int h = ht.x;
     const AttnTile c = a.tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,

@@ -117,7 +117,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     using V8 = typename Vec8<T>::type;
     constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2, kBlock = NARROW ? 32 : 64;   // (a wave's keys of a step)
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
-    const int2 ht = head_tile(bid, a.n_q, a.n_heads);
+    const int2 ht = head_tile(bid, a.n_q, a.n_heads, a.causal);
     const int h = ht.x;
     const AttnTile c = a.q_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
@@ -339,7 +339,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
     float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][kStep]: -L2 (without a cap by am) and -delta of a step's queries
     float* tab = rows + 4 * kStep;
-    const int2 ht = head_tile(bid, a.n_k, a.n_kv * a.head_parts);
+    const int2 ht = head_tile(bid, a.n_k, a.n_kv * a.head_parts, a.causal);
     const int kvh = ht.x / a.head_parts, hp = ht.x - kvh * a.head_parts;
     const int hg0 = hp * a.group / a.head_parts, heads = (hp + 1) * a.group / a.head_parts - hg0, h0 = kvh * a.group + hg0;
     const AttnTile c = a.k_tiles[ht.y];
