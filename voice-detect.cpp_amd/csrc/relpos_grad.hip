@@ -607,23 +607,25 @@ GradCut cut_of(const vdk_attn_plan* p, int radius) {
 // The blocks' partial sums of 64 distances, 16 rows of blocks at a time, in a fixed order.
 __global__ __launch_bounds__(1024) void relpos_dbias_kernel(GradArgs a) {
     __shared__ double red[16][64];
-    const int R = a.radius, h = blockIdx.y, i = blockIdx.x * 64 + (threadIdx.x & 63), row = threadIdx.x >> 6;
+    const int R = a.radius, h = blockIdx.y, i = blockIdx.x * 64 + (threadIdx.x & 63);
+    const int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (so that the spans are scalar loads)
     double sum = 0.0;
-    if (i <= 2 * R) {
-        const bool edge = i == 0 || i == 2 * R;
-        const float* p = a.part + (long long)h * a.n_rows * (2 * R + 1) + i;
-        for (int b0 = row; b0 < a.n_rows; b0 += 16 * 8) {   // eight loads at a time
-            float v[8];
+    const bool edge = i == 0 || i == 2 * R;
+    const int d = i <= 2 * R ? i - R : 1 << 30;
+    const float* p = a.part + (long long)h * a.n_rows * (2 * R + 1) + min(i, 2 * R);
+    for (int b0 = row; b0 < a.n_rows; b0 += 16 * 8) {   // eight loads at a time
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int b = min(b0 + 16 * j, a.n_rows - 1);
+        for (int j = 0; j < 8; ++j) {
+            const int b = b0 + 16 * j;
+            v[j] = 0.0f;
+            if (b < a.n_rows) {
                 const int2 s = a.span[b];
-                const bool ok = b0 + 16 * j < a.n_rows && (edge || (i - R >= s.x && i - R <= s.y));
-                v[j] = ok ? p[(long long)b * (2 * R + 1)] : 0.0f;
+                if (edge || (d >= s.x && d <= s.y)) v[j] = p[(long long)b * (2 * R + 1)];
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += v[j];
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += v[j];
     }
     red[row][threadIdx.x & 63] = sum;
     __syncthreads();
