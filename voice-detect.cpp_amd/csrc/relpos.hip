@@ -106,8 +106,10 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) kf[kk] = at.row_block(tk, kt, kk);
             float16v s = splat16(0.0f);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) s = mfma32(kf[kk], qf[kk], s);
+            __builtin_amdgcn_s_setprio(0);
             // the first values' loads run beside the exponentials
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt) vf[dt] = at.col_block(tv, 2 * kt, dt);
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
                 sum = exponentials(No{});
             }
             l += sum;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -212,6 +215,7 @@ __global__ __launch_bounds__(256, D == 128 || NARROW ? 2 : CAP ? 3 : 4) void rel
                     for (int i = 0; i < kParts; ++i) o[dt] = mfma32(vf[dt], pb[cc][i], o[dt]);
                     if (cc == 0) vf[dt] = at.col_block(tv, 2 * kt + 1, dt);
                 }
+            __builtin_amdgcn_s_setprio(0);
         }
     };
     for (int kb = 0; kb < kend; kb += 2 * kStep) {
