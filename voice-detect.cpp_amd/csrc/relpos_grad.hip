@@ -353,11 +353,22 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
 
     const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + (c.k0 + kr) * a.v_tok + (long long)kvh * a.v_head;
+    // At 64 dims three of the eight pieces of K and V wait in LDS, a lane's own 16 bytes each: the registers of three
+    // workgroups a CU do not hold them, and a spilled one comes back through the counter of the DMAs, so it waits for all
+    // of them (2 x 4096 causal 560 us a training step with spills, 545 so; two workgroups a CU 570).
+    constexpr bool kPark = D == 64 && !NARROW;
+    const int R = BIAS ? a.radius : 0;
+    V8* park = reinterpret_cast<V8*>(BIAS ? tab + 2 * R + 1 + 2 * kTabPad + (3 - (2 * R + 2 * kTabPad) % 4) : tab) + threadIdx.x;
     V8 kf[D / 16], vf[D / 16];
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
         kf[kk] = *reinterpret_cast<const V8*>(kp + 16 * kk + 8 * hl);
         vf[kk] = *reinterpret_cast<const V8*>(vp + 16 * kk + 8 * hl);
+    }
+    if constexpr (kPark) {
+        park[0] = vf[D / 16 - 2];
+        park[256] = vf[D / 16 - 1];
+        park[512] = kf[D / 16 - 1];
     }
     const uint32_t qb_row = (uint32_t)a.q_tok * 2, db_row = (uint32_t)a.do_tok * 2;
     TileDma<D, kStep, NW> dmq, dmo;
@@ -391,7 +402,6 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         }
     };
     if (steps > 0) fetch(0, 0);
-    const int R = BIAS ? a.radius : 0;
 
     float16v dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -440,22 +450,24 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
             const int qs = q + 32 * (NARROW ? wave : qt);
             if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
             // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki.  The sums start from the rows' own terms
-            float16v s, p;
+            auto start = [&](const float* from) {
+                float16v x;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4v l4 = *reinterpret_cast<const float4v*>(nl + 32 * qt + 8 * g + 4 * hl);
-                const float4v d4 = *reinterpret_cast<const float4v*>(nd + 32 * qt + 8 * g + 4 * hl);
+                for (int g = 0; g < 4; ++g) {
+                    const float4v x4 = *reinterpret_cast<const float4v*>(from + 32 * qt + 8 * g + 4 * hl);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[4 * g + e] = CAP ? 0.0f : l4[e];
-                    p[4 * g + e] = d4[e];
+                    for (int e = 0; e < 4; ++e) x[4 * g + e] = x4[e];
                 }
-            }
+                return x;
+            };
+            float16v s = CAP ? splat16(0.0f) : start(nl);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kf[kk], s);
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kPark && kk == D / 16 - 1 ? park[512] : kf[kk], s);
             __builtin_amdgcn_sched_barrier(0);
+            float16v p = start(nd);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(to, qt, kk), vf[kk], p);
+            for (int kk = 0; kk < D / 16; ++kk)
+                p = mfma32(at.row_block(to, qt, kk), kPark && kk >= D / 16 - 2 ? park[256 * (kk & 1)] : vf[kk], p);
             score_w<CAP>(s, a.map);
             const int d0 = kw - (qs + past);   // distances d0 - 31 .. d0 + 31
             const bool near = BIAS && d0 + 31 > -R && d0 - 31 < R;
@@ -589,8 +601,10 @@ struct GradCut {
 };
 
 GradCut cut_of(const vdk_attn_plan* p, int radius) {
-    const int bias = radius ? 4 * (2 * radius + 1 + 2 * kTabPad) + 16 + 4 * 512 * 4 : 0;
-    const int narrow = 8 * kKeys * p->dim * 2 + 2048 + bias, wide = 4 * kKeys * p->dim * 2 + 1024 + bias;
+    const int tab = radius ? 4 * (2 * radius + 1 + 2 * kTabPad) + 16 : 0, ring = radius ? 4 * 512 * 4 : 0;
+    const int park = p->dim == 64 ? 3 * 256 * 16 : 0;   // (dkv_tile's, where dq_tile has its ring)
+    const int narrow = 8 * kKeys * p->dim * 2 + 2048 + tab + ring;
+    const int wide = 4 * kKeys * p->dim * 2 + 1024 + tab + std::max(ring, park);
     GradCut c;
     // Smaller tiles where those of 128 queries leave most CUs idle.  At 64 dims to one for every second CU: 96 tiles (one
     // clip of 1500, 8 heads) 60 us against 73, 48 tiles 103 against 141; 240 tiles of short clips 39 against 30.  At 128
