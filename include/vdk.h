@@ -592,8 +592,9 @@ int vdk_time_mean_states(const void* d_x, size_t state_stride, int n_states, int
  * With `causal` query i sees the keys with r <= 0 and the clip's first `prefix`
  * keys, else all keys of its clip.  A row that sees nothing (no key, or a bias
  * of -inf at each) gives o = 0 and lse = -inf.  A NaN or an infinity in a key
- * or value reaches every query of the same 32 that sees a key of its 64-key
- * tile; clips never reach each other.
+ * or value may reach every query that shares its 32 with one that sees a key of
+ * its tile of 64, also a query that does not see the key; clips never reach
+ * each other.
  *
  * The clips lie one after the other: clip c has queries q_offsets[c] ..
  * q_offsets[c + 1] - 1 and keys kv_offsets[c] .. kv_offsets[c + 1] - 1 (host
