@@ -159,6 +159,14 @@ GRAD += WIDE[:2] + [
     dict(nq=[300, 40, 129], H=16, kv=2, D=128, dtype="f16", causal=True, R=70, cap=25.0),
     dict(nq=[33, 190, 70], nk=[100, 190, 40], H=16, kv=16, D=128, dtype="bf16", R=30),
 ]
+# (enough workgroups at 128 dims for two a CU)
+SHORT = [33, 1, 64, 70, 130, 2, 31, 32, 65, 96, 5, 17, 50, 0, 40]
+GRAD += [
+    dict(nq=SHORT, H=32, kv=8, D=128, dtype="f16", R=40),
+    dict(nq=SHORT, H=32, kv=8, D=128, dtype="bf16", causal=True, prefix=[n // 3 for n in SHORT], cap=20.0, R=800),
+    dict(nq=SHORT, nk=[n + 3 * (n % 40) for n in SHORT], H=32, kv=32, D=128, dtype="bf16", cap=300.0),
+    dict(nq=SHORT, nk=[max(n - 20, 0) for n in SHORT], H=32, kv=8, D=128, dtype="f16", causal=True),
+]
 
 
 @pytest.mark.parametrize("case", GRAD, ids=ident)

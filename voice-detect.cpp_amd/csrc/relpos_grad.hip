@@ -43,6 +43,24 @@ __device__ __forceinline__ float scale_of(float most) {
     return __builtin_amdgcn_ldexpf(1.0f, -11 - e);
 }
 
+// Shapes of a launch: 128 queries (keys) a workgroup, 32 of them a wave; NARROW: 32
+// a workgroup, whose waves share its keys (queries); ROOMY (128 dims): as WIDE, but
+// one workgroup a CU, all the registers it asks for and 64 queries a step.
+enum { WIDE, NARROW, ROOMY };
+
+// dkv_tile: blocks of 32 queries a wave and step, and how many of the 16-byte
+// pieces of a lane's values and keys are kept in LDS, so that the rest fits the
+// registers of three workgroups a CU (128 dims: two).  A spilled one would come
+// back through the counter of the DMAs, and wait for all of them.  At 64 dims 2 x
+// 4096 causal 560 us a training step with spills, 545 so, two workgroups a CU 570;
+// at 128 dims 22 clips of 127-323, 16 heads, 163 us with one workgroup a CU, 134 so.
+template <int D, int SHAPE>
+constexpr int kGradBlocks = SHAPE == NARROW || (SHAPE == WIDE && D == 128) ? 1 : 2;
+template <int D, int SHAPE>
+constexpr int kParkedV = SHAPE != WIDE ? 0 : D == 64 ? 2 : 8;
+template <int SHAPE>
+constexpr int kParkedK = SHAPE != WIDE ? 0 : 1;
+
 template <class T>
 constexpr bool kScaled = std::is_same_v<T, half_t>;
 
@@ -116,20 +134,20 @@ __global__ __launch_bounds__(256) void relpos_delta_kernel(GradArgs a) {
 // dQ and the bias's gradient: one workgroup 128 queries of a head, a wave 32, 64
 // keys a step through double-buffered LDS tiles; S^T and dP^T leave a query's dS
 // in one lane pair, packed as it stands into the operand of dQ^T += K^T dS^T.
-template <class T, int D, bool CAP, bool BIAS, bool NARROW>
+template <class T, int D, bool CAP, bool BIAS, bool kNarrow>
 __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
-    constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2, kBlock = NARROW ? 32 : 64;   // (a wave's keys of a step)
+    constexpr int NW = 4, kStep = kNarrow ? 128 : kKeys, kTile = kStep * D * 2, kBlock = kNarrow ? 32 : 64;   // (a wave's keys of a step)
     float* tab = reinterpret_cast<float*>(smem + 4 * kTile);
     const int2 ht = head_tile(bid, a.n_q, a.n_heads, a.causal);
     const int h = ht.x;
     const AttnTile c = a.q_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, qw = c.row + (NARROW ? 0 : 32 * wave), qi = qw + lr;
+    const int past = c.nk - c.nq, qw = c.row + (kNarrow ? 0 : 32 * wave), qi = qw + lr;
     const int qr = qi < c.nq ? qi : c.nq - 1;
     auto last = [&](int q) { return a.causal ? min(c.nk, max(c.prefix, past + q + 1)) : c.nk; };
-    const int kend = max(last(min(c.row + (NARROW ? 32 : 32 * NW), c.nq) - 1), 0);
+    const int kend = max(last(min(c.row + (kNarrow ? 32 : 32 * NW), c.nq) - 1), 0);
     const int kend_w = qw < c.nq ? last(min(qw + 32, c.nq) - 1) : 0;
     const int kfull = qw < c.nq ? last(qw) : 0;
     const int lim = last(qr);
@@ -169,7 +187,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     float far_l = 0.0f, far_r = 0.0f;
     if constexpr (BIAS) {
         const float* b = a.bias + (long long)h * (2 * R + 1);
-        const int i0 = max(R + kTabPad - 32 - (past + c.row + (NARROW ? 32 : 128)), 0);
+        const int i0 = max(R + kTabPad - 32 - (past + c.row + (kNarrow ? 32 : 128)), 0);
         const int i1 = min(R + kTabPad + 96 + kend - (past + c.row), 2 * R + 1 + 2 * kTabPad);
         for (int i = i0 + threadIdx.x; i < i1; i += 64 * NW)   // (the distances that the tile reaches)
             tab[i] = bias2_of(b[min(max(i - kTabPad, 0), 2 * R)]);
@@ -181,7 +199,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     float acc[5] = {0, 0, 0, 0, 0}, left = 0.0f, right = 0.0f;
     int lo = 1 << 30, hi = -(1 << 30);
     float* part = nullptr;
-    const int row = NARROW ? 4 * (c.b32 + (qw >> 5)) + wave : c.b32 + (qw >> 5);
+    const int row = kNarrow ? 4 * (c.b32 + (qw >> 5)) + wave : c.b32 + (qw >> 5);
     if constexpr (BIAS) {
         part = a.part + ((long long)h * a.n_rows + row) * (2 * R + 1);
 #pragma unroll
@@ -189,11 +207,11 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     }
     // acc[0..3] hold all that their 16 lanes add to the 64 distances from d0 - 15 (+ 4 hl - 16 (lr / 16)): stored, and
     // the 64 distances from d0 - 31, which no later tile reaches, summed over the four sixteens and written out.
-    // (NARROW: a wave's blocks lie 128 distances apart, so each is written whole, zeros up to the next.)
+    // (kNarrow: a wave's blocks lie 128 distances apart, so each is written whole, zeros up to the next.)
     auto flush = [&](int d0) {
         const int rho = lane >> 4, off = 4 * hl - 16 * (rho & 1) - (lane & 15);
 #pragma unroll
-        for (int j = 0; j < (NARROW ? 5 : 4); ++j) ring[128 * rho + ((d0 + off + 16 * j) & 127)] = acc[j];
+        for (int j = 0; j < (kNarrow ? 5 : 4); ++j) ring[128 * rho + ((d0 + off + 16 * j) & 127)] = acc[j];
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         const int d = d0 - 31 + lane;
@@ -205,8 +223,8 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
         if (d <= -R) left += v;
         else if (d >= R) right += v;
         else part[d + R] = v;
-        if (NARROW && d + 64 > -R && d + 64 < R) part[d + 64 + R] = 0.0f;
-        acc[0] = NARROW ? 0.0f : acc[4];
+        if (kNarrow && d + 64 > -R && d + 64 < R) part[d + 64 + R] = 0.0f;
+        acc[0] = kNarrow ? 0.0f : acc[4];
         acc[1] = acc[2] = acc[3] = acc[4] = 0.0f;
     };
 
@@ -215,13 +233,13 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     for (int dt = 0; dt < D / 32; ++dt) dq[dt] = splat16(0.0f);
     const float am = a.map.am;
     TileReads<T, D> at;
-    at.init(smem + (NARROW ? wave * (64 * D) : 0), lane);
+    at.init(smem + (kNarrow ? wave * (64 * D) : 0), lane);
     const float unscale = kScaled<T> ? 1.0f / sc * 0x1p-8f : 1.0f;   // of dS, per row (a power of two)
     for (int k0 = 0, buf = 0; k0 < kend; k0 += kStep, buf ^= 1) {
         wait_vmcnt<0>();
         lds_barrier();
         if (k0 + kStep < kend) fetch(k0 + kStep, buf ^ 1);
-        const int kb = k0 + (NARROW ? 32 * wave : 0);
+        const int kb = k0 + (kNarrow ? 32 * wave : 0);
         if (kb >= kend_w) continue;
         const int tk = buf * 2 * kTile, tv = tk + kTile;
         const int d0 = kb - (qw + past);
@@ -286,7 +304,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
                 lo = min(lo, d0 - 31);
                 hi = d0 + 96;
                 flush(d0);
-                if (!NARROW && (kb + kKeys >= kend_w || d0 + 64 - 31 >= R)) flush(d0 + 64);   // the last one: what is left
+                if (!kNarrow && (kb + kKeys >= kend_w || d0 + 64 - 31 >= R)) flush(d0 + 64);   // the last one: what is left
             }
         }
     }
@@ -305,7 +323,7 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
         }
     }
     float* js = reinterpret_cast<float*>(smem);   // [wave][register][lane]
-    if constexpr (NARROW) {
+    if constexpr (kNarrow) {
         __syncthreads();   // the tiles are no longer read
 #pragma unroll
         for (int r = 0; r < D / 2; ++r) js[(wave * (D / 2) + r) * 64 + lane] = dq[r >> 4][r & 15];
@@ -314,14 +332,14 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     if (qi >= c.nq) return;
     const float f = a.scale * 0x1p-8f / sc;   // undo 2^8 and sc (both powers of two)
     T* out = static_cast<T*>(a.dq) + (c.q0 + qi) * a.dq_tok + (long long)h * a.dq_head;
-    constexpr int kOut = NARROW ? D / 32 : D / 8;   // a wave's groups of four registers
+    constexpr int kOut = kNarrow ? D / 32 : D / 8;   // a wave's groups of four registers
 #pragma unroll
     for (int j = 0; j < kOut; ++j) {
-        const int i = NARROW ? wave * kOut + j : j;
+        const int i = kNarrow ? wave * kOut + j : j;
         float4v v = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if constexpr (NARROW) {
+            if constexpr (kNarrow) {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) v[e] += js[(w * (D / 2) + 4 * i + e) * 64 + lane];
             } else {
@@ -334,17 +352,18 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
     }
 }
 
-// dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 queries a step
+// dK and dV: one workgroup 128 keys of a key head, a wave 32; 64 or 32 queries a step
 // through LDS, the heads that share the keys one after the other, or a part of
 // them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
 // Bound by chains of dependent products and LDS reads at the 2.4 waves a SIMD that
 // 168 registers leave, and with a cap by VALU issue: both kinds of tiles together
 // 140 us at 16 ragged clips of 149-799 frames (VALU 43 %, MFMA 26 %), 380 us at
 // 2 x 4096 causal, capped (VALU 69 %, MFMA 28 %).
-template <class T, int D, bool CAP, bool BIAS, bool NARROW>
+template <class T, int D, bool CAP, bool BIAS, int SHAPE>
 __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
-    constexpr int NW = 4, kStep = NARROW ? 128 : kKeys, kTile = kStep * D * 2;
+    constexpr bool kNarrow = SHAPE == NARROW;
+    constexpr int NW = 4, kBlocks = kGradBlocks<D, SHAPE>, kStep = kNarrow ? 128 : 32 * kBlocks, kTile = kStep * D * 2;
     float* rows = reinterpret_cast<float*>(smem + 4 * kTile);   // [2][2][kStep]: -L2 (without a cap by am) and -delta of a step's queries
     float* tab = rows + 4 * kStep;
     const int2 ht = head_tile(bid, a.n_k, a.n_kv * a.head_parts, a.causal);
@@ -353,7 +372,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     const AttnTile c = a.k_tiles[ht.y];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31,
               hl = lane >> 5;
-    const int past = c.nk - c.nq, kw = c.row + (NARROW ? 0 : 32 * wave), ki = kw + lr;
+    const int past = c.nk - c.nq, kw = c.row + (kNarrow ? 0 : 32 * wave), ki = kw + lr;
     const int kr = ki < c.nk ? ki : c.nk - 1;
     // the first query that sees a key of the tile, down to a whole step
     const int q_first = a.causal && c.row >= c.prefix ? max(c.row - past, 0) & ~63 : 0;
@@ -361,10 +380,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
 
     const T* kp = static_cast<const T*>(a.k) + (c.k0 + kr) * a.k_tok + (long long)kvh * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + (c.k0 + kr) * a.v_tok + (long long)kvh * a.v_head;
-    // At 64 dims three of the eight pieces of K and V wait in LDS, a lane's own 16 bytes each: the registers of three
-    // workgroups a CU do not hold them, and a spilled one comes back through the counter of the DMAs, so it waits for all
-    // of them (2 x 4096 causal 560 us a training step with spills, 545 so; two workgroups a CU 570).
-    constexpr bool kPark = D == 64 && !NARROW;
+    constexpr int kParkV = kParkedV<D, SHAPE>, kParkK = kParkedK<SHAPE>;
     const int R = BIAS ? a.radius : 0;
     V8* park = reinterpret_cast<V8*>(BIAS ? tab + 2 * R + 1 + 2 * kTabPad + (3 - (2 * R + 2 * kTabPad) % 4) : tab) + threadIdx.x;
     V8 kf[D / 16], vf[D / 16];
@@ -373,11 +389,12 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         kf[kk] = *reinterpret_cast<const V8*>(kp + 16 * kk + 8 * hl);
         vf[kk] = *reinterpret_cast<const V8*>(vp + 16 * kk + 8 * hl);
     }
-    if constexpr (kPark) {
-        park[0] = vf[D / 16 - 2];
-        park[256] = vf[D / 16 - 1];
-        park[512] = kf[D / 16 - 1];
-    }
+#pragma unroll
+    for (int i = 0; i < kParkV; ++i) park[256 * i] = vf[D / 16 - kParkV + i];
+#pragma unroll
+    for (int i = 0; i < kParkK; ++i) park[256 * (kParkV + i)] = kf[D / 16 - kParkK + i];
+    auto k_of = [&](int kk) { return kk < D / 16 - kParkK ? kf[kk] : park[256 * (kParkV + kk - (D / 16 - kParkK))]; };
+    auto v_of = [&](int kk) { return kk < D / 16 - kParkV ? vf[kk] : park[256 * (kk - (D / 16 - kParkV))]; };
     const uint32_t qb_row = (uint32_t)a.q_tok * 2, db_row = (uint32_t)a.do_tok * 2;
     TileDma<D, kStep, NW> dmq, dmo;
     dmq.init(qb_row, wave, lane);
@@ -385,12 +402,12 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     float row_v = 0.0f;   // this thread's entry of the next step's rows[]
     auto step_scale = [&](int h, int q) {   // from the largest |dO| of the step's (the wave's) queries
         if constexpr (!kScaled<T>) return 1.0f;
-        if constexpr (NARROW) {
+        if constexpr (kNarrow) {
             q += 32 * wave;
             return q < c.nq ? scale_of(a.most[h * a.n_b32 + c.b32 + (q >> 5)]) : 1.0f;
         }
         const float* p = a.most + h * a.n_b32 + c.b32 + (q >> 5);
-        return scale_of(q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
+        return scale_of(kBlocks == 2 && q + 32 < c.nq ? fmaxf(p[0], p[1]) : p[0]);
     };
     auto fetch = [&](int it, int buf) {
         const int h = h0 + it / per_head, q = q_first + (it % per_head) * kStep;
@@ -416,7 +433,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = splat16(0.0f);
     const float am = a.map.am;
     TileReads<T, D> at;
-    at.init(smem + (NARROW ? wave * (64 * D) : 0), lane);
+    at.init(smem + (kNarrow ? wave * (64 * D) : 0), lane);
     float sc = 1.0f, far_l = 0.0f, far_r = 0.0f;
     if constexpr (kScaled<T>) {
         if (steps > 0) sc = step_scale(h0, q_first);
@@ -438,7 +455,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         if (threadIdx.x < 2 * kStep) rows[buf * 2 * kStep + threadIdx.x] = row_v;
         wait_vmcnt<0>();
         lds_barrier();
-        const float* nl = rows + buf * 2 * kStep + (NARROW ? 32 * wave : 0);
+        const float* nl = rows + buf * 2 * kStep + (kNarrow ? 32 * wave : 0);
         const float* nd = nl + kStep;
         if (it + 1 < steps) fetch(it + 1, buf ^ 1);
         if constexpr (kScaled<T>) {   // dK is carried in the scale of the step: moved with it, exactly
@@ -454,8 +471,8 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
         }
         const int tq = buf * 2 * kTile, to = tq + kTile;
 #pragma unroll
-        for (int qt = 0; qt < (NARROW ? 1 : 2); ++qt) {
-            const int qs = q + 32 * (NARROW ? wave : qt);
+        for (int qt = 0; qt < kBlocks; ++qt) {
+            const int qs = q + 32 * (kNarrow ? wave : qt);
             if (qs >= c.nq || (a.causal && kw >= max(c.prefix, past + min(qs + 32, c.nq)))) continue;
             // register r: query qs + 8 (r / 4) + 4 hl + r % 4, lane: key ki.  The sums start from the rows' own terms
             auto start = [&](const float* from) {
@@ -470,12 +487,11 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
             };
             float16v s = CAP ? splat16(0.0f) : start(nl);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), kPark && kk == D / 16 - 1 ? park[512] : kf[kk], s);
+            for (int kk = 0; kk < D / 16; ++kk) s = mfma32(at.row_block(tq, qt, kk), k_of(kk), s);
             __builtin_amdgcn_sched_barrier(0);
             float16v p = start(nd);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-                p = mfma32(at.row_block(to, qt, kk), kPark && kk >= D / 16 - 2 ? park[256 * (kk & 1)] : vf[kk], p);
+            for (int kk = 0; kk < D / 16; ++kk) p = mfma32(at.row_block(to, qt, kk), v_of(kk), p);
             score_w<CAP>(s, a.map);
             const int d0 = kw - (qs + past);   // distances d0 - 31 .. d0 + 31
             const bool near = BIAS && d0 + 31 > -R && d0 - 31 < R;
@@ -526,7 +542,7 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     }
     const float f = a.scale * 0x1p-8f / sc;
     float* js = reinterpret_cast<float*>(smem);   // [wave][dK's and dV's registers][lane]
-    if constexpr (NARROW) {
+    if constexpr (kNarrow) {
         __syncthreads();   // the tiles are no longer read
 #pragma unroll
         for (int r = 0; r < D / 2; ++r) {
@@ -539,14 +555,14 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
     float* parts = a.kv_part + (((long long)hp * 2 * a.total_kv + c.k0 + ki) * a.n_kv + kvh) * D;
     T* ok = static_cast<T*>(a.dk) + (c.k0 + ki) * a.dk_tok + (long long)kvh * a.dk_head;
     T* ov = static_cast<T*>(a.dv) + (c.k0 + ki) * a.dv_tok + (long long)kvh * a.dv_head;
-    constexpr int kOut = NARROW ? D / 16 : D / 4;   // a wave's groups of four registers, dK's and dV's
+    constexpr int kOut = kNarrow ? D / 16 : D / 4;   // a wave's groups of four registers, dK's and dV's
 #pragma unroll
     for (int j = 0; j < kOut; ++j) {
-        const int i = NARROW ? wave * kOut + j : j, of = i >= D / 8, g = of ? i - D / 8 : i;
+        const int i = kNarrow ? wave * kOut + j : j, of = i >= D / 8, g = of ? i - D / 8 : i;
         float4v v = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if constexpr (NARROW) {
+            if constexpr (kNarrow) {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) v[e] += js[(w * D + 4 * i + e) * 64 + lane];
             } else {
@@ -564,15 +580,14 @@ __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* sm
 }
 
 // Both in one launch, the longer tiles of dK and dV first: the tiles of one fill the chip while the other's last ones run.
-// NARROW: 32 queries (keys) a workgroup, whose waves share its keys (queries).
-template <class T, int D, bool CAP, bool BIAS, bool NARROW>
-__global__ __launch_bounds__(256, D == 128 ? 1 : NARROW ? 2 : 3) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
+template <class T, int D, bool CAP, bool BIAS, int SHAPE>
+__global__ __launch_bounds__(256, (D == 64 ? 3 : 2) - (SHAPE != WIDE)) void relpos_grad_kernel(GradArgs a, int n_dkv, int n_dkv8) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int b = blockIdx.x;
     if (b < n_dkv8) {   // (n_dkv up to a multiple of 8, so that both parts start at the same XCD)
-        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS, NARROW>(a, b, smem);
+        if (b < n_dkv) dkv_tile<T, D, CAP, BIAS, SHAPE>(a, b, smem);
     } else {
-        dq_tile<T, D, CAP, BIAS, NARROW>(a, b - n_dkv8, smem);
+        dq_tile<T, D, CAP, BIAS, SHAPE == NARROW>(a, b - n_dkv8, smem);
     }
 }
 
@@ -606,25 +621,31 @@ __global__ __launch_bounds__(256) void relpos_dkv_join_kernel(GradArgs a) {
 // How a layout's backward pass is cut.
 struct GradCut {
     bool narrow;
+    int shape;
     int head_parts;    // workgroups that share the heads of a key head
     int lds, rows;     // rows of partial sums of the bias's gradient
 };
 
 GradCut cut_of(const vdk_attn_plan* p, int radius) {
     const int tab = radius ? 4 * (2 * radius + 1 + 2 * kTabPad) + 16 : 0, ring = radius ? 4 * 512 * 4 : 0;
-    const int park = p->dim == 64 ? 3 * 256 * 16 : 0;   // (dkv_tile's, where dq_tile has its ring)
-    const int narrow = 8 * kKeys * p->dim * 2 + 2048 + tab + ring;
-    const int wide = 4 * kKeys * p->dim * 2 + 1024 + tab + std::max(ring, park);
+    const int row = p->dim * 2, narrow = 8 * kKeys * row + 2048 + tab + ring, roomy = 4 * kKeys * row + 1024 + tab + ring;
+    const int step = 32 * (p->dim == 64 ? kGradBlocks<64, WIDE> : kGradBlocks<128, WIDE>);
+    const int park = ((p->dim == 64 ? kParkedV<64, WIDE> : kParkedV<128, WIDE>) + kParkedK<WIDE>) * 256 * 16;
+    const int wide = std::max(4 * kKeys * row + tab + ring, 4 * step * row + 16 * step + tab + park);
     GradCut c;
     // Smaller tiles where those of 128 queries leave most CUs idle.  At 64 dims to one for every second CU: 96 tiles (one
     // clip of 1500, 8 heads) 60 us against 73, 48 tiles 103 against 141; 240 tiles of short clips 39 against 30.  At 128
     // dims, where one workgroup fills a CU's LDS, far fewer: 32 tiles 77 us against 119, 60 tiles 135 against 111.
     c.narrow = (long long)p->n_q128 * p->n_heads <= (p->dim == 64 ? 128 : 32) && narrow <= 163840;
-    c.lds = c.narrow ? narrow : wide;
     c.rows = p->n_b32 * (c.narrow ? 4 : 1);
     // 1024 workgroups (narrow: 512) fill the chip twice, and causal tiles differ most in their work where they are few
     const long long groups = std::max(1ll, (long long)(c.narrow ? p->n_k32 : p->n_k128) * p->n_kv);
     c.head_parts = (int)std::max(1ll, std::min<long long>(p->n_heads / p->n_kv, ((c.narrow ? 512 : 1024) + groups - 1) / groups));
+    // One workgroup a CU at 128 dims where all are few: 512 of them (2 x 2000 causal, 8 heads) 178 us against 217, 1024 (2 x
+    // 2048 causal, 16 heads) 353 against 294.
+    const long long all = groups * c.head_parts + (long long)p->n_q128 * p->n_heads;
+    c.shape = c.narrow ? NARROW : p->dim == 128 && all < 768 ? ROOMY : WIDE;
+    c.lds = c.narrow ? narrow : c.shape == ROOMY ? roomy : wide;
     return c;
 }
 
@@ -674,10 +695,14 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, const GradCut& cut, hipStre
     const long long n_dkv = (long long)a.n_k * a.n_kv * a.head_parts, n_dkv8 = (n_dkv + 7) / 8 * 8;
     const long long n = n_dkv8 + (long long)a.n_q * a.n_heads;
     if (n > 0) {
-        cut.narrow ? allow_lds<relpos_grad_kernel<T, D, CAP, BIAS, true>>(cut.lds)
-                   : allow_lds<relpos_grad_kernel<T, D, CAP, BIAS, false>>(cut.lds);
-        auto kern = cut.narrow ? relpos_grad_kernel<T, D, CAP, BIAS, true> : relpos_grad_kernel<T, D, CAP, BIAS, false>;
-        hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), cut.lds, s, a, (int)n_dkv, (int)n_dkv8);
+        auto go = [&](auto shape) {
+            constexpr auto kern = relpos_grad_kernel<T, D, CAP, BIAS, shape.value>;
+            allow_lds<kern>(cut.lds);
+            hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(256), cut.lds, s, a, (int)n_dkv, (int)n_dkv8);
+        };
+        if (cut.shape == NARROW) go(std::integral_constant<int, NARROW>{});
+        else if (D == 64 || cut.shape == WIDE) go(std::integral_constant<int, WIDE>{});
+        else go(std::integral_constant<int, D == 64 ? WIDE : ROOMY>{});
         VDK_HIP(hipGetLastError());
         if (a.head_parts > 1) {
             const long long threads = a.total_kv * a.n_kv * (D / 8);
