@@ -638,9 +638,13 @@ GradCut cut_of(const vdk_attn_plan* p, int radius) {
     // dims, where one workgroup fills a CU's LDS, far fewer: 32 tiles 77 us against 119, 60 tiles 135 against 111.
     c.narrow = (long long)p->n_q128 * p->n_heads <= (p->dim == 64 ? 128 : 32) && narrow <= 163840;
     c.rows = p->n_b32 * (c.narrow ? 4 : 1);
-    // 1024 workgroups (narrow: 512) fill the chip twice, and causal tiles differ most in their work where they are few
+    // The heads of a key head are split up to 512 workgroups of dK and dV, the tiles of dQ beside them; causal tiles, which
+    // differ in their work, up to 1024 (2 x 4096 545 us a training step against 566).  More parts cost their sums: 57 clips
+    // of 64-90 frames, 16 heads on 2, in 8 parts 143 us, in 4 124; 22 clips of 127-323, 16 on 4, in 4 parts 179, in 2 160.
     const long long groups = std::max(1ll, (long long)(c.narrow ? p->n_k32 : p->n_k128) * p->n_kv);
-    c.head_parts = (int)std::max(1ll, std::min<long long>(p->n_heads / p->n_kv, ((c.narrow ? 512 : 1024) + groups - 1) / groups));
+    const int share = p->n_heads / p->n_kv, most = p->causal && !c.narrow ? 1024 : 512;
+    c.head_parts = (int)std::min<long long>(share, (most + groups - 1) / groups);
+    c.head_parts = cdiv(share, cdiv(share, c.head_parts));   // (no more than the largest part needs)
     // One workgroup a CU at 128 dims where all are few: 512 of them (2 x 2000 causal, 8 heads) 178 us against 217, 1024 (2 x
     // 2048 causal, 16 heads) 353 against 294.
     const long long all = groups * c.head_parts + (long long)p->n_q128 * p->n_heads;
