@@ -357,8 +357,8 @@ __device__ __forceinline__ void dq_tile(const GradArgs& a, int bid, uint8_t* sme
 // them each workgroup and the parts' sums added up by relpos_dkv_join_kernel.
 // Bound by chains of dependent products and LDS reads at the 2.4 waves a SIMD that
 // 168 registers leave, and with a cap by VALU issue: both kinds of tiles together
-// 140 us at 16 ragged clips of 149-799 frames (VALU 43 %, MFMA 26 %), 380 us at
-// 2 x 4096 causal, capped (VALU 69 %, MFMA 28 %).
+// 138 us at 16 ragged clips of 149-799 frames (VALU 44 %, MFMA 27 %), 371 us at
+// 2 x 4096 causal, capped (VALU 73 %, MFMA 30 %).
 template <class T, int D, bool CAP, bool BIAS, int SHAPE>
 __device__ __forceinline__ void dkv_tile(const GradArgs& a, int bid, uint8_t* smem) {
     using V8 = typename Vec8<T>::type;
