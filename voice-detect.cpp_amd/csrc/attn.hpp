@@ -216,7 +216,7 @@ struct ScoreMap {
 };
 
 constexpr float kTanhC[3] = {1.0f, -0.33331817f, 0.13153109f};
-constexpr float kTanhD[5] = {1.0f, -0.33333072f, 0.13324828f, -0.05298924f, 0.01714132f};
+constexpr float kTanhD[5] = {1.0f, -0.33333071f, 0.13324828f, -0.05298924f, 0.01714132f};
 
 inline ScoreMap score_map(float scale, float cap) {
     ScoreMap m{1.0f, scale * kLog2e, {}, {}, {}};
