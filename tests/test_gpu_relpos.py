@@ -167,6 +167,12 @@ GRAD += [
     dict(nq=SHORT, nk=[n + 3 * (n % 40) for n in SHORT], H=32, kv=32, D=128, dtype="bf16", cap=300.0),
     dict(nq=SHORT, nk=[max(n - 20, 0) for n in SHORT], H=32, kv=8, D=128, dtype="f16", causal=True),
 ]
+# (no key at all, no query at all, with shared heads)
+GRAD += [
+    dict(nq=[5, 40], nk=[0, 0], H=4, kv=1, D=64, dtype="f16", R=5),
+    dict(nq=[200], nk=[0], H=64, kv=8, D=128, dtype="bf16", causal=True),
+    dict(nq=[0, 0], nk=[3, 140], H=4, kv=2, D=128, dtype="f16", R=5),
+]
 
 
 @pytest.mark.parametrize("case", GRAD, ids=ident)

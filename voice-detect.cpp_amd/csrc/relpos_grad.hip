@@ -708,7 +708,7 @@ void launch_grad(const vdk_attn_plan* p, GradArgs a, const GradCut& cut, hipStre
         else if (D == 64 || cut.shape == WIDE) go(std::integral_constant<int, WIDE>{});
         else go(std::integral_constant<int, D == 64 ? WIDE : ROOMY>{});
         VDK_HIP(hipGetLastError());
-        if (a.head_parts > 1) {
+        if (a.head_parts > 1 && a.total_kv > 0) {
             const long long threads = a.total_kv * a.n_kv * (D / 8);
             hipLaunchKernelGGL((relpos_dkv_join_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, s, a);
             VDK_HIP(hipGetLastError());
